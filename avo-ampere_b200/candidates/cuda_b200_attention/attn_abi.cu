@@ -19,6 +19,7 @@
 
 #include "attn_fwd.cuh"
 #include "avo_b200_attn.h"
+#include "host_common.h"
 
 namespace avo_b200 {
 
@@ -319,7 +320,7 @@ const PlanEntry& cached_plan(int num_bh, int seq_q, int seq_kv, int causal, long
 int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int num_bh,
                int seq_q, int seq_kv, int head_dim, long long q_hs, long long kv_hs, long long o_hs,
                long long lse_hs, int causal, float scale, long long q_pos0, long long kv_pos0,
-               int* status, void* stream, void* workspace = nullptr, size_t workspace_bytes = 0) {
+               int* status, void* stream, void* workspace = nullptr, size_t workspace_bytes = 0, int kv_group = 1) {
   if (q == nullptr || k == nullptr || v == nullptr || o == nullptr) return AVO_B200_EINVAL;
   if (head_dim != kHeadDim || num_bh < 0 || seq_q < 0 || seq_kv < 0) return AVO_B200_EINVAL;
   if (!(scale > 0.f) || !std::isfinite(scale)) return AVO_B200_EINVAL;
@@ -353,8 +354,8 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
   alignas(64) CUtensorMap tm_q, tm_k, tm_v;
   const int kv_rows = seq_kv > 0 ? seq_kv : 1;  // never read when seq_kv == 0
   if ((rc = encode_rows(&tm_q, q, seq_q, num_bh, q_hs)) != AVO_B200_OK) return rc;
-  if ((rc = encode_rows(&tm_k, k, kv_rows, num_bh, kv_hs)) != AVO_B200_OK) return rc;
-  if ((rc = encode_rows(&tm_v, v, kv_rows, num_bh, kv_hs)) != AVO_B200_OK) return rc;
+  if ((rc = encode_rows(&tm_k, k, kv_rows, num_bh / kv_group, kv_hs)) != AVO_B200_OK) return rc;
+  if ((rc = encode_rows(&tm_v, v, kv_rows, num_bh / kv_group, kv_hs)) != AVO_B200_OK) return rc;
 
   AttnParams p{};
   p.plan = plan;
@@ -377,6 +378,7 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
   p.seq_q = seq_q;
   p.seq_kv = seq_kv;
   p.num_bh = num_bh;
+  p.kv_group = kv_group;
   p.causal = causal ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
 
@@ -422,6 +424,15 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
 }
 
 }  // namespace
+
+namespace host {
+unsigned long long watchdog_limit() { return watchdog_limit_ns(); }
+int skip_load() { return test_skip_load(); }
+int device(int* sm_count) { return prepare_device(sm_count); }
+int encode(CUtensorMap* map, const void* base, int rows, int heads) {
+  return encode_rows(map, base, rows, heads, static_cast<long long>(rows) * kHeadDim);
+}
+}  // namespace host
 }  // namespace avo_b200
 
 using namespace avo_b200;
@@ -454,6 +465,20 @@ extern "C" int avo_b200_attn_fwd(const void* q, const void* k, const void* v, vo
   const long long hs = static_cast<long long>(seq) * kHeadDim;
   return launch_fwd(q, k, v, o, lse, static_cast<int>(bh), seq, seq, head_dim, hs, hs, hs, seq, causal,
                     softmax_scale, 0, 0, status_dev, stream);
+}
+
+extern "C" int avo_b200_attn_fwd_grouped(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
+                                         int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
+                                         float softmax_scale, int* status_dev, void* stream) {
+  if (batch < 0 || heads < 0 || kv_heads <= 0 || seq_q < 0 || seq_kv < 0 || heads % kv_heads != 0)
+    return AVO_B200_EINVAL;
+  const long long bh = static_cast<long long>(batch) * heads;
+  if (bh > INT_MAX) return AVO_B200_EINVAL;
+  const long long qhs = static_cast<long long>(seq_q) * kHeadDim, khs = static_cast<long long>(seq_kv) * kHeadDim;
+  // Query row i sits at position seq_kv - seq_q + i: the last query sees every key.
+  return launch_fwd(q, k, v, o, lse, static_cast<int>(bh), seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim, qhs,
+                    seq_q, causal, softmax_scale, static_cast<long long>(seq_kv) - seq_q, 0, status_dev, stream,
+                    nullptr, 0, heads > 0 ? heads / kv_heads : 1);
 }
 
 extern "C" int avo_b200_attn_workspace_size(size_t* bytes) {

@@ -131,6 +131,7 @@ struct AttnParams {
   int seq_q;
   int seq_kv;
   int num_bh;
+  int kv_group;                 // query heads per key/value head: pair bh reads head bh / kv_group
   void* o;                      // bf16 output rows, [num_bh, o_head_stride]
   int o_sector_aligned;         // o and o_head_stride * 2 bytes are multiples of 32
   long long o_head_stride;      // elements between consecutive heads of o
@@ -803,6 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d(sQ + i * kTileBytes + h * kHalfBytes, &tm_q, bar(BAR_Q), h * 64, u.q0 + i * kBlockM,
                         u.bh, pol_q);
         ++nq;
+        const int kv_bh = u.bh / p.kv_group;
         for (int lt = 0; lt < 2 * n_tiles; ++lt, ++tt) {
           const int slot = tt % kStages;
           const int use = tt / kStages;
@@ -822,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int krow = (u.t0 + (lt >> 1)) * kBlockN;
           for (int h = 0; h < 2; ++h)
             tma_load_3d(sRing + slot * kTileBytes + h * kHalfBytes, tm, bar(BAR_KV_FULL + slot), h * 64, krow,
-                        u.bh, pol_kv);
+                        kv_bh, pol_kv);
           last_copy = (last_copy & ~(3u << (2 * slot))) | ((1u | ((use & 1u) << 1)) << (2 * slot));
         }
       }

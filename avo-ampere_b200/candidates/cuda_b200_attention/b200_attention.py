@@ -55,6 +55,18 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _c_int,
         [_c_int, _c_int, _c_int, _c_int, _c_ll, _c_ll, _c_int, _c_int, _vp, _vp, _c_int, _vp],
     ),
+    "avo_b200_attn_fwd_grouped": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, _vp],
+    ),
+    "avo_b200_attn_bwd_workspace_size": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "avo_b200_attn_bwd": (
+        _c_int,
+        [_vp] * 9 + [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, ctypes.c_size_t, _vp, _vp],
+    ),
     "avo_b200_attn_fwd_split_noalloc": (
         _c_int,
         [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _vp, _vp],

@@ -10,6 +10,11 @@ and dtype, as ``torch::empty_like`` gives in the reference seeds
 Additive export ``attention_with_lse(q, k, v, causal) -> (O, LSE)`` returns the fp32
 natural-log LSE ``[B, H, S]`` as well.
 
+For training, ``grouped_attention(q, k, v, causal) -> (O, LSE)`` is the forward with shared
+key/value heads and separate query and key lengths, differentiable by autograd, and
+``attention_backward(dO, q, k, v, O, LSE, causal) -> (dq, dk, dv)`` its gradient as a plain
+call.
+
 The kernel lives in the companion directory ``cuda_b200_attention/`` (TMA +
 tcgen05/TMEM, warp-specialised, built ahead of time by nvcc for sm_100a and called
 through a C ABI).  There is no CPU or eager fallback.
@@ -23,26 +28,39 @@ from pathlib import Path
 
 _DIR = Path(__file__).resolve().parent / "cuda_b200_attention"
 _BINDING = "avo_b200_attention_binding"
+_TRAINING = "avo_b200_training_binding"
 
 AVO_SOURCE_FILES = (
     "cuda_b200_attention/sm100_ptx.cuh",
     "cuda_b200_attention/schedule.cuh",
     "cuda_b200_attention/attn_fwd.cuh",
+    "cuda_b200_attention/attn_bwd.cuh",
+    "cuda_b200_attention/host_common.h",
     "cuda_b200_attention/attn_abi.cu",
+    "cuda_b200_attention/attn_bwd.cu",
     "cuda_b200_attention/fast_call.c",
     "cuda_b200_attention/b200_attention.py",
+    "cuda_b200_attention/b200_training.py",
     "cuda_b200_attention/build.py",
 )
 
 
-def _binding():
-    module = sys.modules.get(_BINDING)
+def _load(name: str, file: str):
+    module = sys.modules.get(name)
     if module is None:
-        spec = importlib.util.spec_from_file_location(_BINDING, _DIR / "b200_attention.py")
+        spec = importlib.util.spec_from_file_location(name, _DIR / file)
         module = importlib.util.module_from_spec(spec)
-        sys.modules[_BINDING] = module
+        sys.modules[name] = module
         spec.loader.exec_module(module)
     return module
+
+
+def _binding():
+    return _load(_BINDING, "b200_attention.py")
+
+
+def _training():
+    return _load(_TRAINING, "b200_training.py")
 
 
 def attention(q, k, v, causal: bool):
@@ -52,3 +70,13 @@ def attention(q, k, v, causal: bool):
 
 def attention_with_lse(q, k, v, causal: bool):
     return _binding().attention_forward(q, k, v, causal, need_lse=True)
+
+
+def grouped_attention(q, k, v, causal: bool, *, softmax_scale: float | None = None):
+    return _training().grouped_attention(q, k, v, causal, softmax_scale=softmax_scale)
+
+
+def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: float | None = None, dq=None,
+                       dk=None, dv=None):
+    return _training().attention_backward(dout, q, k, v, out, lse, causal, softmax_scale=softmax_scale, dq=dq,
+                                          dk=dk, dv=dv)

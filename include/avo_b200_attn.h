@@ -172,6 +172,37 @@ int avo_b200_attn_fwd_split_noalloc(const void* q, const void* k, const void* v,
                                     float softmax_scale, int n_splits, int* status_dev, void* stream);
 
 /*
+ * Attention forward with shared key/value heads and separate lengths: q and o are
+ * [batch, heads, seq_q, 128], k and v [batch, kv_heads, seq_kv, 128], heads a multiple of
+ * kv_heads (query head h reads key/value head h / (heads / kv_heads)); lse is fp32
+ * [batch, heads, seq_q] and may be null.  causal != 0 aligns the two sequences at their
+ * ends: query i sees keys j <= i + seq_kv - seq_q, so with seq_q > seq_kv the first
+ * queries see none (o = 0, lse = -inf).  Whole work items only, no workspace: calls on
+ * several streams share nothing.  No reference counterpart.
+ */
+int avo_b200_attn_fwd_grouped(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
+                              int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
+                              float softmax_scale, int* status_dev, void* stream);
+
+/*
+ * Gradient of avo_b200_attn_fwd_grouped (and, with kv_heads == heads and seq_kv == seq_q,
+ * of avo_b200_attn_fwd): given dout, the forward's inputs and its o and lse, writes dq like
+ * q, and dk and dv like k (summed over the query heads that share a key/value head), all
+ * bf16.  The probabilities are recomputed from q, k and lse.  The same inputs give the same
+ * bits in every call: nothing is accumulated in an order that can change.
+ * dq, dk, dv must be 32-byte aligned, the inputs 16-byte aligned.
+ * workspace: device memory of avo_b200_attn_bwd_workspace_size() bytes, 256-byte aligned,
+ * uninitialised; used from the launch until the call's work on the stream is done.  Calls
+ * that may overlap in time need a workspace each.  No reference counterpart (the reference
+ * scores the forward only).
+ */
+int avo_b200_attn_bwd_workspace_size(int batch, int heads, int kv_heads, int seq_q, int seq_kv, size_t* bytes);
+int avo_b200_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o,
+                      const float* lse, void* dq, void* dk, void* dv, int batch, int heads, int kv_heads,
+                      int seq_q, int seq_kv, int head_dim, int causal, float softmax_scale, void* workspace,
+                      size_t workspace_bytes, int* status_dev, void* stream);
+
+/*
  * Self-test of the device watchdog without faulting the GPU: one CTA waits on an
  * mbarrier that nothing ever completes, with the given limit in microseconds; the
  * wait expires, the kernel sets AVO_B200_STATUS_WATCHDOG in *status_dev and returns.
