@@ -24,8 +24,12 @@ from typing import Any
 
 HERE = Path(__file__).resolve().parent
 
-# Every function declared in include/avo_b200_attn.h, with (restype, argtypes).
 _c_int, _c_ll, _c_float, _vp = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+# The arguments that both directions of the QKV norm + rotation share, from `batch` to `eps`.
+_ROPE_ARGS = [_c_int] * 5 + [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _c_ll, _c_ll, _c_ll,
+                            _c_int, _vp, _c_float]
+
+# Every function declared in include/avo_b200_attn.h, with (restype, argtypes).
 SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "avo_b200_abi_version": (_c_int, []),
     "avo_b200_strerror": (ctypes.c_char_p, [_c_int]),
@@ -67,6 +71,12 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _c_int,
         [_vp] * 9 + [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, ctypes.c_size_t, _vp, _vp],
     ),
+    "avo_b200_qkv_norm_rope": (_c_int, [_vp, _c_ll, _c_ll, _vp, _vp, _vp, *_ROPE_ARGS, _vp, _vp]),
+    "avo_b200_qkv_norm_rope_bwd_workspace_size": (_c_int, [ctypes.POINTER(ctypes.c_size_t)]),
+    "avo_b200_qkv_norm_rope_bwd": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_ll, _c_ll, _vp, _vp, _vp, *_ROPE_ARGS, _vp, ctypes.c_size_t, _vp, _vp],
+    ),
     "avo_b200_attn_fwd_split_noalloc": (
         _c_int,
         [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _vp, _vp],
@@ -76,6 +86,7 @@ ABI_VERSION = 1
 HEAD_DIM = 128
 STATUS_WATCHDOG = 1
 STATUS_DRAIN = 2
+STATUS_POSITION = 4
 NOALLOC_MAX_ROWS = 16384  # AVO_B200_NOALLOC_MAX_ROWS
 ETOOBIG = 6
 EREGS = 7
@@ -242,6 +253,10 @@ def check_status(device, *, reset: bool = True) -> int:
         raise B200AttentionError(
             f"device watchdog fired (status {value}): a kernel pipeline wait timed out; "
             "outputs of that launch are invalid"
+        )
+    if value & STATUS_POSITION:
+        raise B200AttentionError(
+            f"a position lies outside the cos/sin table (status {value}): the rotated values of its token are NaN"
         )
     return value
 

@@ -1,4 +1,4 @@
-"""The training side of attention: shared key/value heads and the gradient.
+"""The training side of attention: its input stage, shared key/value heads and the gradients.
 
 Host side of the entry points of include/avo_b200_attn.h that the forward contract does not
 cover, in the manner of b200_attention.py (argument checks that raise ``RuntimeError``, the
@@ -6,7 +6,10 @@ current CUDA stream of the tensors' device, the device's status word, no fallbac
 
 * ``grouped_attention``: the forward with H query heads over Hkv key/value heads and
   seq_q != seq_kv, differentiable through torch's autograd;
-* ``attention_backward``: its gradient as a plain call.
+* ``attention_backward``: its gradient as a plain call;
+* ``qkv_norm_rope``: from a fused projection to attention's q, k, v (norms of queries and
+  keys, rotary positions on one or several axes, heads in front of tokens), differentiable;
+* ``qkv_norm_rope_backward``: its gradient as a plain call.
 
 Scratch is allocated per call by torch's caching allocator on the current stream, so calls
 on several streams, and several captured graphs, share nothing but the status word.
@@ -215,3 +218,206 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
             scale, scratch.data_ptr(), size.value, b.status_word(index).data_ptr(), b._raw_stream(index))
     b._check(code, "avo_b200_attn_bwd")
     return tuple(grads)
+
+
+# ---------------------------------------------------------------- QKV norm + rotation
+MAX_AXES = 4
+
+
+def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved):
+    """Checks the arguments both directions share; (batch, seq, device arguments of the C
+    calls from `batch` to `eps`, what they point to)."""
+    torch = _torch()
+    if not qkv.is_cuda:
+        raise RuntimeError("qkv must be a CUDA tensor")
+    if qkv.dtype != torch.bfloat16:
+        raise RuntimeError("qkv must be bf16")
+    if heads < 0 or kv_heads < 0:
+        raise RuntimeError("the numbers of heads must not be negative")
+    if qkv.dim() != 4 or qkv.shape[2] != heads + 2 * kv_heads or qkv.shape[3] != HEAD_DIM:
+        raise RuntimeError(f"qkv must have shape (batch, seq, heads + 2 * kv_heads, {HEAD_DIM})")
+    batch, seq = qkv.shape[0], qkv.shape[1]
+    if qkv.numel() and (qkv.stride(3) != 1 or (qkv.shape[2] > 1 and qkv.stride(2) != HEAD_DIM)):
+        raise RuntimeError("the heads of a token of qkv must be contiguous")
+    _check_tensors((("cos", cos), ("sin", sin)), torch.float32, qkv.device)
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise RuntimeError("cos and sin must have the same shape (positions, rotary_dim / 2)")
+    rotary = 2 * cos.shape[1]
+    if rotary == 0 or rotary > HEAD_DIM or rotary % 16 != 0:
+        raise RuntimeError(f"rotary_dim must be a multiple of 16 up to {HEAD_DIM}")
+    if (q_weight is None) != (k_weight is None):
+        raise RuntimeError("q_weight and k_weight must be given together")
+    if q_weight is not None:
+        if q_weight.dtype not in (torch.float32, torch.bfloat16):
+            raise RuntimeError("q_weight must be fp32 or bf16")
+        _check_tensors((("q_weight", q_weight), ("k_weight", k_weight)), q_weight.dtype, qkv.device)
+        if tuple(q_weight.shape) != (HEAD_DIM,) or tuple(k_weight.shape) != (HEAD_DIM,):
+            raise RuntimeError(f"q_weight and k_weight must have shape ({HEAD_DIM},)")
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise RuntimeError("eps must not be negative")
+    axes, section_array, strides = 1, None, (0, 0, 0)
+    if sections is not None:
+        sections = [int(n) for n in sections]
+        axes = len(sections)
+        if not 1 <= axes <= MAX_AXES or any(n < 0 for n in sections) or sum(sections) != rotary // 2:
+            raise RuntimeError(f"sections must be 1 to {MAX_AXES} counts that sum to rotary_dim / 2")
+        if positions is None:
+            raise RuntimeError("sections need positions")
+        section_array = (ctypes.c_int * axes)(*sections)
+    if positions is None:
+        if seq > cos.shape[0]:
+            raise RuntimeError("cos and sin have fewer rows than the sequence has tokens")
+    else:
+        if not positions.is_cuda or positions.device != qkv.device:
+            raise RuntimeError("positions must be on the device of qkv")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError("positions must be int32 or int64")
+        shape = tuple(positions.shape) if sections is None else tuple(positions.shape[1:])
+        if shape not in ((seq,), (batch, seq)) or (sections is not None and positions.shape[0] != axes):
+            lead = "" if sections is None else "axes, "
+            raise RuntimeError(f"positions must have shape ({lead}seq) or ({lead}batch, seq)")
+        if cos.shape[0] == 0 and positions.numel():
+            raise RuntimeError("cos and sin have no rows")
+        at = positions.stride()
+        strides = (at[0] if sections is not None else 0, at[-2] if len(shape) == 2 else 0, at[-1])
+    args = [batch, seq, heads, kv_heads, HEAD_DIM,
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+            int(q_weight is not None and q_weight.dtype == torch.bfloat16), cos.data_ptr(), sin.data_ptr(),
+            cos.shape[0], rotary, 1 if interleaved else 0, None if positions is None else positions.data_ptr(),
+            int(positions is not None and positions.dtype == torch.int64), *strides, axes,
+            None if section_array is None else ctypes.addressof(section_array), eps]
+    return batch, seq, args, section_array
+
+
+def _qkv_strides(qkv) -> tuple[int, int]:
+    """Batch and token stride (a dimension of one element has no stride to speak of)."""
+    return (qkv.stride(0) if qkv.shape[0] > 1 else 0), (qkv.stride(1) if qkv.shape[1] > 1 else 0)
+
+
+def _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved):
+    torch = _torch()
+    batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
+                                        interleaved)
+    q, k, v = (torch.empty((batch, n, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
+               for n in (heads, kv_heads, kv_heads))
+    if qkv.numel() == 0:
+        return q, k, v
+    lib = b.load_library()
+    index = qkv.get_device()
+    with _on(index):
+        code = lib.avo_b200_qkv_norm_rope(qkv.data_ptr(), *_qkv_strides(qkv), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                          *args, b.status_word(index).data_ptr(), b._raw_stream(index))
+    del keep
+    b._check(code, "avo_b200_qkv_norm_rope")
+    return q, k, v
+
+
+def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight=None, positions=None, sections=None,
+                           eps: float = 1e-6, interleaved: bool = False):
+    """(dqkv, dq_weight, dk_weight) of ``qkv_norm_rope`` for the gradients of its outputs.
+
+    dq is bf16 [B, H, S, 128], dk and dv [B, Hkv, S, 128], contiguous; qkv and the other
+    arguments are the forward's.  dqkv is a new contiguous tensor of qkv's shape, the weight
+    gradients are fp32 [128] (None without weights).  Equal inputs give equal bits."""
+    torch = _torch()
+    _check_tensors((("dq", dq), ("dk", dk), ("dv", dv)), torch.bfloat16, qkv.device)
+    if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape:
+        raise RuntimeError("dq, dk and dv must have shape (batch, heads, seq, dim), dk and dv the same")
+    heads, kv_heads = dq.shape[1], dk.shape[1]
+    batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
+                                        interleaved)
+    if tuple(dq.shape) != (batch, heads, seq, HEAD_DIM) or tuple(dk.shape) != (batch, kv_heads, seq, HEAD_DIM):
+        raise RuntimeError("dq, dk and dv must match qkv's batch and sequence")
+    dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+    lib = b.load_library()
+    index = qkv.get_device()
+    with _on(index):
+        weights, scratch, size = (None, None), None, 0
+        if q_weight is not None:
+            weights = tuple(torch.empty(HEAD_DIM, dtype=torch.float32, device=qkv.device) for _ in range(2))
+            size = _rope_scratch_bytes(index)
+            scratch = torch.empty(size, dtype=torch.uint8, device=qkv.device)
+        code = lib.avo_b200_qkv_norm_rope_bwd(
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), *_qkv_strides(qkv),
+            dqkv.data_ptr(), *(None if w is None else w.data_ptr() for w in weights), *args,
+            None if scratch is None else scratch.data_ptr(), size, b.status_word(index).data_ptr(),
+            b._raw_stream(index))
+    del keep
+    b._check(code, "avo_b200_qkv_norm_rope_bwd")
+    return (dqkv, *weights)
+
+
+_rope_scratch: dict[int, int] = {}
+
+
+def _rope_scratch_bytes(index: int) -> int:
+    """Scratch of the backward on device ``index`` (a function of the device alone)."""
+    if index not in _rope_scratch:
+        size = ctypes.c_size_t(0)
+        b._check(b.load_library().avo_b200_qkv_norm_rope_bwd_workspace_size(ctypes.byref(size)),
+                 "avo_b200_qkv_norm_rope_bwd_workspace_size")
+        _rope_scratch[index] = size.value
+    return _rope_scratch[index]
+
+
+def _norm_rope_function():
+    fn = _autograd_functions.get("norm_rope")
+    if fn is not None:
+        return fn
+    torch = _torch()
+
+    class QkvNormRope(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, qkv, q_weight, k_weight, cos, sin, positions, heads, kv_heads, sections, eps, interleaved):
+            ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin, positions)
+            ctx.how = (sections, eps, interleaved)
+            return _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dq, dk, dv):
+            qkv, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+            sections, eps, interleaved = ctx.how
+            with _on(qkv.get_device()):
+                _refuse_capture("the backward of qkv_norm_rope")
+            dqkv, dqw, dkw = qkv_norm_rope_backward(
+                dq.contiguous(), dk.contiguous(), dv.contiguous(), qkv, cos, sin, q_weight=q_weight,
+                k_weight=k_weight, positions=positions, sections=sections, eps=eps, interleaved=interleaved)
+            if dqw is not None:
+                dqw, dkw = dqw.to(q_weight.dtype), dkw.to(k_weight.dtype)
+            return (dqkv, dqw, dkw, *([None] * 8))
+
+    _autograd_functions["norm_rope"] = QkvNormRope
+    return QkvNormRope
+
+
+def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=None, k_weight=None, positions=None,
+                  sections=None, eps: float = 1e-6, interleaved: bool = False):
+    """(q, k, v) for attention from a fused projection, in one pass.
+
+    qkv is bf16 [B, S, H + 2 Hkv, 128]: query, key and value heads of each token (batch and
+    token strides are free).  Query and key heads are divided by their root mean square
+    (with ``eps``) and multiplied by ``q_weight`` / ``k_weight`` ([128], fp32 or bf16; both
+    None: no norm), then their first R values are rotated by the fp32 tables ``cos`` and
+    ``sin`` [P, R / 2]: pair f is (f, f + R / 2), or (2 f, 2 f + 1) when ``interleaved``.
+    q is bf16 [B, H, S, 128], k and v [B, Hkv, S, 128], contiguous.
+
+    ``positions`` (int32 or int64) are the table rows: [S] or [B, S]; None is 0..S-1.  With
+    ``sections`` (how many consecutive pairs each axis turns, up to 4 axes), positions are
+    [axes, S] or [axes, B, S].  A position outside the table makes the token's rotated values
+    NaN and is reported by ``check_status()``.
+
+    With gradients enabled and an input that requires them, the result is differentiable in
+    qkv and the weights (once); such a call cannot be captured in a CUDA graph: capture the
+    call under ``torch.no_grad()`` and ``qkv_norm_rope_backward``."""
+    torch = _torch()
+    sections = None if sections is None else tuple(int(n) for n in sections)
+    heads, kv_heads, interleaved = int(num_heads), int(num_kv_heads), bool(interleaved)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
+        _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved)
+        with _on(qkv.get_device()):
+            _refuse_capture("qkv_norm_rope")
+        return _norm_rope_function().apply(qkv, q_weight, k_weight, cos, sin, positions, heads, kv_heads, sections,
+                                           float(eps), interleaved)
+    return _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved)

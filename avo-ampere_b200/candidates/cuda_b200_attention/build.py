@@ -23,8 +23,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 LIB_NAME = "libavo_b200_attn.so"
 LIB_PATH = HERE / LIB_NAME
-SOURCES = ("attn_abi.cu", "attn_bwd.cu")
-HEADERS = ("attn_fwd.cuh", "attn_bwd.cuh", "host_common.h", "sm100_ptx.cuh", "schedule.cuh")
+SOURCES = ("attn_abi.cu", "attn_bwd.cu", "qkv_norm_rope.cu")
+HEADERS = ("attn_fwd.cuh", "attn_bwd.cuh", "qkv_norm_rope.cuh", "host_common.h", "sm100_ptx.cuh", "schedule.cuh")
 GENCODE = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = (
     *GENCODE,

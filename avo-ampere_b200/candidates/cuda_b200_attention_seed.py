@@ -13,7 +13,9 @@ natural-log LSE ``[B, H, S]`` as well.
 For training, ``grouped_attention(q, k, v, causal) -> (O, LSE)`` is the forward with shared
 key/value heads and separate query and key lengths, differentiable by autograd, and
 ``attention_backward(dO, q, k, v, O, LSE, causal) -> (dq, dk, dv)`` its gradient as a plain
-call.
+call; ``qkv_norm_rope(qkv, H, Hkv, cos, sin, ...) -> (q, k, v)`` makes attention's inputs from
+a fused projection (norms of queries and keys, rotary positions, layout) and
+``qkv_norm_rope_backward`` is its gradient.
 
 The kernel lives in the companion directory ``cuda_b200_attention/`` (TMA +
 tcgen05/TMEM, warp-specialised, built ahead of time by nvcc for sm_100a and called
@@ -35,9 +37,11 @@ AVO_SOURCE_FILES = (
     "cuda_b200_attention/schedule.cuh",
     "cuda_b200_attention/attn_fwd.cuh",
     "cuda_b200_attention/attn_bwd.cuh",
+    "cuda_b200_attention/qkv_norm_rope.cuh",
     "cuda_b200_attention/host_common.h",
     "cuda_b200_attention/attn_abi.cu",
     "cuda_b200_attention/attn_bwd.cu",
+    "cuda_b200_attention/qkv_norm_rope.cu",
     "cuda_b200_attention/fast_call.c",
     "cuda_b200_attention/b200_attention.py",
     "cuda_b200_attention/b200_training.py",
@@ -80,3 +84,16 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
                        dk=None, dv=None):
     return _training().attention_backward(dout, q, k, v, out, lse, causal, softmax_scale=softmax_scale, dq=dq,
                                           dk=dk, dv=dv)
+
+
+def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=None, k_weight=None, positions=None,
+                  sections=None, eps: float = 1e-6, interleaved: bool = False):
+    return _training().qkv_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=q_weight, k_weight=k_weight,
+                                     positions=positions, sections=sections, eps=eps, interleaved=interleaved)
+
+
+def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight=None, positions=None, sections=None,
+                           eps: float = 1e-6, interleaved: bool = False):
+    return _training().qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, q_weight=q_weight, k_weight=k_weight,
+                                              positions=positions, sections=sections, eps=eps,
+                                              interleaved=interleaved)

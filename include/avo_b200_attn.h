@@ -32,6 +32,8 @@
  * caller zeroes the word and reads it after synchronizing):
  *   AVO_B200_STATUS_WATCHDOG   1  a pipeline wait exceeded the watchdog; outputs invalid
  *   AVO_B200_STATUS_DRAIN      2  draining in-flight work after an abort also timed out
+ *   AVO_B200_STATUS_POSITION   4  a position lies outside the cos/sin table: the rotated
+ *                                 values (or gradients) of its token are NaN
  */
 #ifndef AVO_B200_ATTN_H_
 #define AVO_B200_ATTN_H_
@@ -57,6 +59,7 @@ extern "C" {
 
 #define AVO_B200_STATUS_WATCHDOG 1
 #define AVO_B200_STATUS_DRAIN 2
+#define AVO_B200_STATUS_POSITION 4
 
 /* ABI revision of this header; bumped on any signature change. */
 int avo_b200_abi_version(void);
@@ -201,6 +204,53 @@ int avo_b200_attn_bwd(const void* dout, const void* q, const void* k, const void
                       const float* lse, void* dq, void* dk, void* dv, int batch, int heads, int kv_heads,
                       int seq_q, int seq_kv, int head_dim, int causal, float softmax_scale, void* workspace,
                       size_t workspace_bytes, int* status_dev, void* stream);
+
+/*
+ * From a fused projection to the inputs of attention in one pass.  qkv is bf16
+ * [batch, seq, heads + 2 * kv_heads, 128] (query heads, key heads, value heads; the last
+ * two dimensions contiguous, token_stride and batch_stride in elements, multiples of 8).
+ * Query and key heads are divided by sqrt(mean square + eps) and multiplied by q_weight or
+ * k_weight ([128], fp32, or bf16 with weight_bf16 != 0; both null: no norm); their first
+ * rotary_dim values (a multiple of 16, at most 128) are rotated: a pair (a, b) becomes
+ * (a cos - b sin, b cos + a sin), where pair f is (f, f + rotary_dim / 2), or
+ * (2 f, 2 f + 1) with interleaved != 0, and cos and sin are column f of row `position` of
+ * the fp32 tables [table_rows, rotary_dim / 2].  Value heads are copied.  Outputs q, k, v:
+ * bf16 [batch, heads or kv_heads, seq, 128] contiguous.
+ *
+ * positions: null (position = token index, seq <= table_rows), or int32 / int64 device
+ * values at axis * pos_axis_stride + batch * pos_batch_stride + token * pos_token_stride
+ * elements.  axes = 1: one position per token.  axes = 2..4: one per axis (time, height,
+ * width, ...); axis a turns sections[a] consecutive pairs (host array; the sections sum to
+ * rotary_dim / 2).  A position outside the table sets AVO_B200_STATUS_POSITION and gives
+ * NaN in the token's rotated values.  batch * seq is limited to 2^31 - 1 tokens.
+ * No reference counterpart (the reference starts at q, k, v).
+ */
+int avo_b200_qkv_norm_rope(const void* qkv, long long batch_stride, long long token_stride, void* q, void* k,
+                           void* v, int batch, int seq, int heads, int kv_heads, int head_dim,
+                           const void* q_weight, const void* k_weight, int weight_bf16, const float* cos,
+                           const float* sin, int table_rows, int rotary_dim, int interleaved,
+                           const void* positions, int positions_int64, long long pos_axis_stride,
+                           long long pos_batch_stride, long long pos_token_stride, int axes,
+                           const int* sections, float eps, int* status_dev, void* stream);
+
+/*
+ * Gradient of avo_b200_qkv_norm_rope: dq, dk, dv like its outputs, qkv and the other
+ * arguments as there; writes dqkv (bf16 [batch, seq, heads + 2 * kv_heads, 128] contiguous)
+ * and, with weights, their gradients dq_weight and dk_weight (fp32 [128] each).  Equal
+ * inputs give equal bits.  workspace (only used with weights): device memory of
+ * avo_b200_qkv_norm_rope_bwd_workspace_size() bytes, 16-byte aligned, uninitialised; calls
+ * that may overlap in time need a workspace each.
+ */
+int avo_b200_qkv_norm_rope_bwd_workspace_size(size_t* bytes);
+int avo_b200_qkv_norm_rope_bwd(const void* dq, const void* dk, const void* dv, const void* qkv,
+                               long long batch_stride, long long token_stride, void* dqkv, float* dq_weight,
+                               float* dk_weight, int batch, int seq, int heads, int kv_heads, int head_dim,
+                               const void* q_weight, const void* k_weight, int weight_bf16, const float* cos,
+                               const float* sin, int table_rows, int rotary_dim, int interleaved,
+                               const void* positions, int positions_int64, long long pos_axis_stride,
+                               long long pos_batch_stride, long long pos_token_stride, int axes,
+                               const int* sections, float eps, void* workspace, size_t workspace_bytes,
+                               int* status_dev, void* stream);
 
 /*
  * Self-test of the device watchdog without faulting the GPU: one CTA waits on an

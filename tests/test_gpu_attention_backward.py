@@ -123,3 +123,260 @@ def test_backward_matches_fp64(b200, training, case):
     for name, g, w, bound in zip(("dq", "dk", "dv"), got, grads, bounds):
         assert g.dtype == torch.bfloat16 and g.shape == w.shape
         assert_within(g, w, bound, name)
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_grouped_forward_matches_fp64(b200, training, case):
+    # O: P rounded to bf16 (the row sum is taken over unrounded P), then O rounded once:
+    # |err| <= sum_j P (u + e) |V| + u |O|.  LSE: the exponentials' relative error and fp32.
+    import torch
+
+    q, k, v, do = make(case, seed=2)
+    out, lse, _, _ = plain(q, k, v, do, case[5], b200.default_scale())
+    got, got_lse = training.grouped_attention(q, k, v, case[5])
+    torch.cuda.synchronize()
+    b200.check_status(q.device)
+    group = case[1] // case[2]
+    kx, vx = (t.double().repeat_interleave(group, 1) for t in (k, v))
+    s = b200.default_scale() * (q.double() @ kx.transpose(-1, -2))
+    if case[5]:
+        i = torch.arange(case[3], device=q.device)[:, None] + case[4] - case[3]
+        s = s.masked_fill(torch.arange(case[4], device=q.device)[None, :] > i, -math.inf)
+    p = torch.where(lse[..., None] == -math.inf, torch.zeros_like(s), torch.exp(s - lse[..., None]))
+    e = 2e-4 + 128 * EPS32 * b200.default_scale() * (q.double().abs() @ kx.abs().transpose(-1, -2))
+    e = e + case[4] * EPS32
+    assert_within(got, out, 2 * ((p * (U + e)) @ vx.abs()) + U * out.abs(), "out")
+    empty = lse == -math.inf
+    assert torch.equal(got_lse == -math.inf, empty) and bool((got[empty] == 0).all())
+    assert float((got_lse.double() - lse)[~empty].abs().max()) <= 1e-3
+
+
+def test_equal_shapes_give_the_candidate_forwards_bits(b200, training):
+    import torch
+
+    for case in [(1, 4, 4, 512, 512, False), (1, 4, 4, 500, 500, True)]:
+        q, k, v, _ = make(case, seed=3)
+        out, lse = training.grouped_attention(q, k, v, case[5])
+        want, want_lse = b200.attention_forward(q, k, v, case[5], split=False)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_rows_without_keys_get_zero_gradients(b200, training):
+    import torch
+
+    case = (1, 2, 1, 300, 100, True)  # rows 0..199 see nothing
+    q, k, v, do = make(case, seed=4)
+    q[:, :, :200] = 1e30   # what no key sees must not matter, however large
+    do[:, :, :200] = 1e30
+    out, lse = training.grouped_attention(q, k, v, True)
+    assert bool((out[:, :, :200] == 0).all()) and bool((lse[:, :, :200] == -math.inf).all())
+    dq, dk, dv = training.attention_backward(do, q, k, v, out, lse, True)
+    tail = [t[:, :, 200:].contiguous() for t in (do, q, out, lse)]
+    dq2, dk2, dv2 = training.attention_backward(tail[0], tail[1], k, v, tail[2], tail[3], True)
+    torch.cuda.synchronize()
+    b200.check_status(q.device)
+    assert bool((dq[:, :, :200] == 0).all())
+    _, _, grads, bounds = plain(tail[1], k, v, tail[0], True, b200.default_scale())
+    for name, g, w, bound in zip(("dq", "dk", "dv"), (dq[:, :, 200:], dk, dv), grads, bounds):
+        assert_within(g, w, 2 * bound, name)  # out and lse are the forward kernel's here
+    for g, h in zip((dk, dv), (dk2, dv2)):
+        assert bool(torch.isfinite(g.float()).all()) and bool(torch.isfinite(h.float()).all())
+
+
+def test_large_scores_and_inputs(b200, training):
+    # k x 3 makes rows peaked: P is then 0 or 1 almost everywhere.
+    import torch
+
+    case = (1, 2, 2, 384, 384, True)
+    q, k, v, do = make(case, seed=5, std_do=1e4)
+    k = (k * 3).contiguous()
+    out, lse, grads, bounds = plain(q, k, v, do, True, b200.default_scale())
+    got = training.attention_backward(do, q, k, v, out.bfloat16(), lse.float(), True)
+    torch.cuda.synchronize()
+    for name, g, w, bound in zip(("dq", "dk", "dv"), got, grads, bounds):
+        assert_within(g, w, bound, name)
+
+
+def test_gradient_against_differences(b200, training):
+    # L(q, k, v) = sum dO . O in fp64: a central difference along a random direction d is
+    # <grad, d> up to the kernel's bound sum |d| bound and the difference's own error
+    # (h^2 / 6 times the third derivative, below 1e-6 of the value at h = 1e-3 here).
+    import torch
+
+    case = (1, 4, 2, 150, 210, True)
+    q, k, v, do = make(case, seed=6)
+    scale = b200.default_scale()
+    out, lse, _, bounds = plain(q, k, v, do, True, scale)
+    got = training.attention_backward(do, q, k, v, out.bfloat16(), lse.float(), True)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    base = [t.double() for t in (q, k, v)]
+    for i in range(3):
+        d = torch.randn(base[i].shape, device="cuda", generator=gen, dtype=torch.float64)
+        value = []
+        for h in (1e-3, -1e-3):
+            x = list(base)
+            x[i] = x[i] + h * d
+            value.append(float((plain(*x, do, True, scale)[0] * do.double()).sum()))
+        slope = (value[0] - value[1]) / 2e-3
+        mine = float((got[i].double() * d).sum())
+        assert abs(mine - slope) <= float((bounds[i] * d.abs()).sum()) + 1e-4 * abs(slope), (i, mine, slope)
+
+
+def test_same_inputs_give_the_same_bits(b200, training):
+    import torch
+
+    case = (2, 8, 2, 900, 900, True)
+    q, k, v, do = make(case, seed=8)
+    out, lse = training.grouped_attention(q, k, v, True)
+    first = training.attention_backward(do, q, k, v, out, lse, True)
+    for _ in range(3):
+        again = training.attention_backward(do, q, k, v, out, lse, True)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+def test_two_streams_at_once(b200, training):
+    import torch
+
+    cases = [(1, 8, 2, 1024, 1024, True), (1, 8, 8, 640, 900, False)]
+    sets, want = [], []
+    for case in cases:
+        q, k, v, do = make(case, seed=9)
+        out, lse = training.grouped_attention(q, k, v, case[5])
+        sets.append((do, q, k, v, out, lse))
+        want.append(training.attention_backward(*sets[-1], case[5]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = training.attention_backward(*sets[i], cases[i][5])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+def test_outputs_into_given_tensors_and_back_to_back_use(b200, training):
+    # The gradients are read by the next work in the stream at once: both passes of the
+    # backward have to be complete by then.
+    import torch
+
+    case = (1, 16, 4, 2048, 2048, True)
+    q, k, v, do = make(case, seed=10)
+    out, lse = training.grouped_attention(q, k, v, True)
+    want = training.attention_backward(do, q, k, v, out, lse, True)
+    torch.cuda.synchronize()
+    grads = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+    for _ in range(5):
+        for g in grads:
+            g.fill_(float("nan"))
+        result = training.attention_backward(do, q, k, v, out, lse, True, dq=grads[0], dk=grads[1], dv=grads[2])
+        copies = [g.clone() for g in grads]
+        # The forward kernel starts early (programmatic launch) behind the backward: it may
+        # only see complete gradients.
+        after, _ = training.grouped_attention(grads[0], grads[1], grads[2], True)
+        torch.cuda.synchronize()
+        assert all(r is g for r, g in zip(result, grads))
+        assert all(torch.equal(c, w) for c, w in zip(copies, want))
+        assert torch.equal(after, training.grouped_attention(want[0], want[1], want[2], True)[0])
+
+
+def test_captured_backward_replays(b200, training):
+    import torch
+
+    case = (1, 8, 4, 700, 700, True)
+    q, k, v, do = make(case, seed=11)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, lse = training.grouped_attention(q, k, v, True)
+        training.attention_backward(do, q, k, v, out, lse, True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):  # two graphs share nothing
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = training.grouped_attention(q, k, v, True)
+            results.append(training.attention_backward(do, q, k, v, out, lse, True))
+        graphs.append(graph)
+    for seed in (12, 13):
+        fresh = make(case, seed=seed)
+        for dst, src in zip((q, k, v, do), fresh):
+            dst.copy_(src)
+        for graph in graphs:
+            graph.replay()
+        nq, nk, nv, ndo = fresh
+        out, lse = training.grouped_attention(nq, nk, nv, True)
+        want = training.attention_backward(ndo, nq, nk, nv, out, lse, True)
+        torch.cuda.synchronize()
+        for got in results:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    del graphs
+
+
+def test_autograd_and_its_refusals(b200, training):
+    import torch
+
+    case = (1, 4, 2, 200, 200, True)
+    q, k, v, do = make(case, seed=14)
+    out, lse = training.grouped_attention(q, k, v, True)
+    want = training.attention_backward(do, q, k, v, out, lse, True)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    got, got_lse = training.grouped_attention(*leaves, True)
+    assert torch.equal(got, out) and not got_lse.requires_grad
+    got.backward(do.transpose(1, 2).contiguous().transpose(1, 2))  # a gradient in another layout
+    assert all(torch.equal(leaf.grad, w) for leaf, w in zip(leaves, want))
+    # A broadcast gradient.
+    for leaf in leaves:
+        leaf.grad = None
+    got, _ = training.grouped_attention(*leaves, True)
+    got.sum().backward()
+    ones = training.attention_backward(torch.ones_like(q), q, k, v, out, lse, True)
+    assert all(torch.equal(leaf.grad, w) for leaf, w in zip(leaves, ones))
+    # Only the log-sum-exp used: no gradient flows, none is invented.
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            training.grouped_attention(*leaves, True)
+        with torch.no_grad():
+            training.grouped_attention(*leaves, True)
+    del graph
+
+
+def test_refusals(b200, training):
+    import torch
+
+    q, k, v, do = make((1, 4, 2, 64, 96, False), seed=15)
+    out, lse = training.grouped_attention(q, k, v, False)
+    bad = [
+        (lambda: training.grouped_attention(q.cpu(), k, v, False), "q must be a CUDA tensor"),
+        (lambda: training.grouped_attention(q.half(), k, v, False), "q must be bf16"),
+        (lambda: training.grouped_attention(q.transpose(1, 2), k, v, False), "q must be contiguous"),
+        (lambda: training.grouped_attention(q[:, :3].contiguous(), k, v, False), "multiple of the key/value heads"),
+        (lambda: training.grouped_attention(q, k, v[:, :, :95].contiguous(), False), "same shape"),
+        (lambda: training.grouped_attention(q, k, v, False, softmax_scale=0.0), "softmax_scale"),
+        (lambda: training.grouped_attention(q[..., :64].contiguous(), k, v, False), "head_dim must be 128"),
+        (lambda: training.attention_backward(do[:, :2].contiguous(), q, k, v, out, lse, False), "dout must have"),
+        (lambda: training.attention_backward(do.float(), q, k, v, out, lse, False), "dout must be bf16"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse[:, :2].contiguous(), False), "lse must have"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse.double(), False), "lse must be float32"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse, False, dk=torch.empty_like(q)), "dk must have"),
+    ]
+    for call, match in bad:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+
+
+def test_empty_sizes(b200, training):
+    import torch
+
+    for shape in [(0, 2, 1, 4, 4), (1, 2, 1, 0, 4), (1, 2, 1, 4, 0), (1, 2, 1, 0, 0)]:
+        q, k, v, do = make((*shape, True), seed=16)
+        out, lse = training.grouped_attention(q, k, v, True)
+        grads = training.attention_backward(do, q, k, v, out, lse, True)
+        torch.cuda.synchronize()
+        assert out.shape == q.shape and lse.shape == q.shape[:3]
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+        for g, like in zip(grads, (q, k, v)):
+            assert g.shape == like.shape and bool((g == 0).all())
