@@ -144,6 +144,7 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
     return AVO_B200_ELAUNCH;
   p.g1 = dq;
   p.g2 = nullptr;
+  p.x1 = q;
   if (!host::launch_early(bwd::attn_bwd_kernel<true>, static_cast<unsigned>(q_items < sms ? q_items : sms),
                           bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
     return AVO_B200_ELAUNCH;

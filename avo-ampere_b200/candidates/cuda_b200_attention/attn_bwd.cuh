@@ -8,36 +8,41 @@
 //
 // Three launches.  stats_kernel writes -LSE*log2(e) and -delta per query row.  Then one
 // kernel template runs twice over 128 x 128 tiles, each time with one side of the tile
-// stationary in shared memory and the other streamed:
+// stationary and the other streamed through shared memory:
 //
 //             rows (M)   stationary X1, X2   streamed Y1, Y2   accumulators in TMEM
 //   dK/dV     keys       K, V                Q, dO             dK += dS^T Q, dV += P^T dO
 //   dQ        queries    Q, dO               K, V              dQ += dS K
 //
 //   T1 = X1 Y1^T (S or S^T), T2 = X2 Y2^T (dP or dP^T); the softmax warps turn them into P
-//   and dS, bf16, in place in TMEM, where they are the A operand of the accumulating MMAs.
+//   and dS, bf16, in TMEM, where they are the A operand of the accumulating MMAs.
 //
 // Two passes recompute S and dP: 7 products per tile pair instead of the 5 that one pass
 // needs.  In exchange dQ is not accumulated across CTAs: no atomics (the result does not
 // depend on the order in which CTAs run), no fp32 dQ in memory, and neither P nor dS ever
-// leaves TMEM.  With one 128 x 128 tile in flight per pass the tensor pipe is what bounds
-// both passes: per tile it needs 2048 (dK/dV) and 1536 (dQ) cycles, and the 256 softmax
-// threads' work on it overlaps, phase against phase:
+// leaves TMEM.  Per tile the tensor pipe needs 2048 (dK/dV) and 1536 (dQ) cycles, and the
+// 256 softmax threads' work on it overlaps, phase against phase:
 //
 //   dK/dV:  tensor   | dV_n  S_{n+1} | dK_n  dP_{n+1} | dV_{n+1} ...
 //           softmax  | dS_n from dP_n | P_{n+1} from S_{n+1} | ...
-//   dQ:     tensor   | dP_{n+1}  dQ_n  S_{n+2} | ...           (S double buffered)
-//           softmax  | P_{n+1} from S_{n+1}, dS_{n+1} from dP_{n+1} | ...
+//   dQ:     tensor   | S_{n+1} | dP_{n+1} | dQ_n | ...
+//           softmax  | P_n from S_n | dS_n from dP_n | P_{n+1} ...
+//
+// In dK/dV, TMEM holds T1, T2 and two accumulators, so P and dS replace T1 and T2 in place
+// and a T is only recomputed once the MMA that reads its P or dS has been issued.  dQ has one
+// accumulator; the free columns hold dS and Q itself (as the A operand of S: one tile less
+// in shared memory and 32 KB less to read from it per tile, which leaves room for a fourth
+// K slot), so S_{n+1} and dP_{n+1} start as soon as S_n and dP_n are in registers.
 //
 // Sums are fp32 in TMEM; P and dS are rounded once to bf16 (the type of the tensor cores'
 // operands: half a step, 2^-9 of each value), the gradients once at the end.
 //
 // Roles (512 threads): warps 0-7 softmax (two warpgroups, 64 of a tile's 128 columns each),
-// warps 8-11 the epilogue (an item's accumulators to memory while the next item's first
-// tiles run), warp 12 TMA producer, warp 13 MMA issuer, warp 14 waiter: the issuer waits on
-// hardware named barriers only, because a shared-memory read by the issuing thread drains
-// its queued MMAs first.  Every wait is bounded by the watchdog, and after an abort every
-// role still takes its fixed number of barrier rounds, so no CTA is left waiting.
+// warps 8-11 the epilogue (an item's accumulators to memory, and Q of the next item to TMEM,
+// while the tile loop runs), warp 12 TMA producer, warp 13 MMA issuer, warp 14 waiter: the
+// issuer waits on hardware named barriers only, because a shared-memory read by the issuing
+// thread drains its queued MMAs first.  Every wait is bounded by the watchdog, and after an
+// abort every role still takes its fixed number of barrier rounds, so no CTA is left waiting.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -63,38 +68,78 @@ constexpr uint32_t kBwdRegsOther = 72;
 static_assert(256 * kBwdRegsSoftmax + 128 * kBwdRegsEpi + 128 * kBwdRegsOther <= kBwdThreads * kBwdRegsLaunch,
               "register split");
 
-// Named barriers: 3 waiter -> issuer, 4 P in TMEM, 5 dS in TMEM (the 8 softmax warps arrive,
-// the issuer syncs), 6 / 7 accumulator 1 / 2 read out (the epilogue warps arrive).
-constexpr uint32_t kBarLoaded = 3;
-constexpr uint32_t kBarP = 4;
-constexpr uint32_t kBarDs = 5;
-constexpr uint32_t kBarAcc1 = 6;
-constexpr uint32_t kBarAcc2 = 7;
+// A wait that lasts as long as an item of `tiles` tiles: one lane polls, asleep in between,
+// so that it takes no issue slots and no shared-memory bandwidth from the tile loop.  Each
+// of the item's tiles has a watchdog of its own, so their sum bounds this wait.
+__device__ __forceinline__ bool wait_item(uint32_t bar, uint32_t parity, int tiles, const Watch& w, int lane) {
+  bool ok = true;
+  if (lane == 0) {
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait_sleep(bar, parity, 20000)) {
+      ok = !*w.abort;
+      if (ok && (global_timer_ns() - t0) / (static_cast<uint64_t>(tiles) + 2) > w.limit_ns) {
+        *w.abort = 1;
+        if (w.status != nullptr) atomicOr(w.status, kStatusWatchdog);
+        ok = false;
+      }
+      if (!ok) break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
 
-// Y1 (used by T1 and by the last MMA of its tile) has three slots and Y2 two: with two Y1
-// slots a tile's load could only start 1024 tensor cycles before its use, about the latency
-// of a 32 KB load.
-constexpr int kY1 = 3;
+// Named barriers, all synced by the issuer.  Those with two ids alternate (by tile, or by
+// item): an arrival is then never counted to a round that the issuer has not reached, also
+// after an abort, when a warp no longer waits for the MMAs that order the rounds.
+//   3             first tile's operands loaded (waiter)
+//   dK/dV: 4/7, 5/8  halves of P in TMEM (8 softmax warps; 5/8: and the waiter, next T1's operand)
+//          6/9       dS in TMEM (softmax, and the waiter: next T2's operand)
+//          10/11, 12/13  accumulator 1 / 2 read out (epilogue warps)
+//   dQ:    4/7, 5/8  T1 / T2 in registers (softmax, and the waiter: next T1's / T2's operand)
+//          6/9       dS in TMEM (softmax)
+//          10/11     accumulator read out, 12/13 next item's Q in TMEM (epilogue warps)
+constexpr uint32_t kBarLoaded = 3;
+enum : uint32_t { kRoundP0 = 4, kRoundP1 = 5, kRoundT1Read = 4, kRoundT2Read = 5, kRoundDs = 6 };
+__device__ __forceinline__ uint32_t bar_tile(uint32_t round, uint32_t tile) { return round + (tile & 1) * 3; }
+__device__ __forceinline__ uint32_t bar_acc1(uint32_t item) { return 10 + (item & 1); }
+__device__ __forceinline__ uint32_t bar_acc2(uint32_t item) { return 12 + (item & 1); }
+__device__ __forceinline__ uint32_t bar_x1(uint32_t item) { return 12 + (item & 1); }
+constexpr uint32_t kHalfThreads = kSoftmaxThreads + 32;   // softmax and issuer
+constexpr uint32_t kTileThreads = kSoftmaxThreads + 64;   // softmax, waiter and issuer
+template <bool kDq>
+constexpr uint32_t kDsThreads = kDq ? kHalfThreads : kTileThreads;
+constexpr uint32_t kEpiThreads = 128 + 32;                // epilogue and issuer
+
+// Shared memory: X1 (dK/dV only), X2, the Y1 slots, two Y2 slots, statistics (dK/dV only).
+// Y1 is used by T1 and by the last MMA of its tile.  With two Y1 slots in dK/dV a tile's load
+// could only start 1024 tensor cycles before its use, about the latency of a 32 KB load.
 constexpr int kY2 = 2;
-constexpr int kSmX1 = 0;
-constexpr int kSmX2 = kTileBytes;
-constexpr int kSmY1 = 2 * kTileBytes;
-constexpr int kSmY2 = kSmY1 + kY1 * kTileBytes;
-constexpr int kSmStat = kSmY2 + kY2 * kTileBytes;  // two slots of [-LSE*log2 e | -delta], 128 floats each
+template <bool kDq>
+struct Smem {
+  static constexpr int kY1 = kDq ? 4 : 3;
+  static constexpr int kX1 = 0;
+  static constexpr int kX2 = kDq ? 0 : kTileBytes;
+  static constexpr int kY1At = kX2 + kTileBytes;
+  static constexpr int kY2At = kY1At + kY1 * kTileBytes;
+  static_assert(kY2At + kY2 * kTileBytes == 7 * kTileBytes, "both passes fill seven tiles");
+};
+constexpr int kSmStat = 7 * kTileBytes;  // two slots of [-LSE*log2 e | -delta], 128 floats each
 constexpr int kStatBytes = 2 * kTile * 4;
 constexpr int kSmBars = kSmStat + 2 * kStatBytes;
+// mbarriers.  The issuer commits after T1 and after T2 of a tile, and these commits also tell
+// the producer that the MMAs issued before them are done with their operands (a commit takes
+// about 50 cycles of the issuer's time).  Only dQ's Y1 slots have a commit of their own.
+// T1_FULL and T2_FULL are pairs, used by even and odd tiles, so that no wait can miss a phase.
 enum : int {
   B_X1_FULL = 0,
+  B_X1_DONE = B_X1_FULL,  // dQ: the item's last S is done with Q in TMEM
   B_X2_FULL,
-  B_X1_EMPTY,
-  B_X2_EMPTY,
   B_Y1_FULL,
-  B_Y1_EMPTY = B_Y1_FULL + kY1,
-  B_Y2_FULL = B_Y1_EMPTY + kY1,
-  B_Y2_EMPTY = B_Y2_FULL + kY2,
-  B_T1_FULL = B_Y2_EMPTY + kY2,  // two: dQ's T1 is double buffered
+  B_Y1_EMPTY = B_Y1_FULL + 4,
+  B_Y2_FULL = B_Y1_EMPTY + 4,
+  B_T1_FULL = B_Y2_FULL + kY2,
   B_T2_FULL = B_T1_FULL + 2,
-  B_ACC1,
+  B_ACC1 = B_T2_FULL + 2,
   B_ACC2,
   B_STAT,
   B_DRAINED = B_STAT + 2,
@@ -105,11 +150,13 @@ constexpr int kSmAbort = kSmTmem + 4;
 constexpr int kBwdSmemBytes = (kSmAbort + 4 + 15) / 16 * 16;
 static_assert(kBwdSmemBytes <= 227 * 1024, "shared memory budget");
 
-// TMEM columns: T1 | T2 | accumulator 1 | accumulator 2 (dK/dV) or T1's second buffer (dQ).
+// TMEM columns: T1 | T2 | accumulator 1 | accumulator 2 (dK/dV) or dS and Q (dQ).
 constexpr uint32_t kColT1 = 0, kColT2 = 128, kColAcc1 = 256, kColAcc2 = 384;
+constexpr uint32_t kColDs = 384, kColX1 = 448;
 
 struct BwdParams {
   const float* stats;  // [num_q_heads][nq][2][128]: -LSE*log2(e), -delta
+  const void* x1;      // dQ: Q, [q_heads, seq_q, 128]
   void* g1;            // dK or dQ
   void* g2;            // dV, or null
   int* status;
@@ -133,6 +180,13 @@ struct Items {
   int head, tile;  // stationary head and tile
   int t0, n;       // first streamed tile, tiles in all (dK/dV: over the whole group of heads)
   __device__ explicit Items(const BwdParams& params) : p(params) {}
+  // The next item that has tiles.
+  __device__ bool next_busy() {
+    do {
+      if (!next()) return false;
+    } while (n == 0);
+    return true;
+  }
   __device__ bool next() {
     const int heads = kDq ? p.q_heads : p.kv_heads;
     const int tiles = kDq ? p.nq : p.nkv;
@@ -183,9 +237,7 @@ struct Tiles {
   __device__ bool next() {
     first = false;
     if (left == 0) {
-      do {
-        if (!items.next()) return false;
-      } while (items.n == 0);
+      if (!items.next_busy()) return false;
       left = items.n;
       first = true;
       t = items.t0;
@@ -208,15 +260,34 @@ __device__ __forceinline__ void issue_xy(uint32_t d_tmem, uint32_t x_lo, uint32_
   issue_qk(d_tmem, x_lo, y_lo, kDescHiSw128);
 }
 
-// acc (+)= A Y over the 128 streamed rows: A (P or dS, bf16) from TMEM, where each softmax
-// warpgroup has put its 64 columns' values at the start of its own half of the tile; Y from
-// shared memory as an MN-major operand.
-__device__ __forceinline__ void issue_acc(uint32_t d_tmem, uint32_t a_tmem, uint32_t y_lo, uint32_t accumulate) {
-  constexpr uint32_t idesc = idesc_bf16_f32(kTile, kHeadDim, 0, 1);
+// The same with X in TMEM.
+__device__ __forceinline__ void issue_xy_tmem(uint32_t d_tmem, uint32_t x_tmem, uint32_t y_lo) {
+  constexpr uint32_t idesc = idesc_bf16_f32(kTile, kTile, 0, 0);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    mma_ts_lo(d_tmem, a_tmem + (kk >> 2) * 64 + (kk & 3) * 8, y_lo + ((kk * 16 * 128) >> 4), kDescHiSw128, idesc,
-              accumulate | (kk > 0 ? 1u : 0u));
+    mma_ts_lo(d_tmem, x_tmem + kk * 8, y_lo + (((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), kDescHiSw128, idesc,
+              kk > 0 ? 1u : 0u);
+}
+
+// acc (+)= A Y over 64 of the 128 streamed rows: A (P or dS, bf16) from TMEM, Y from shared
+// memory as an MN-major operand.  Each softmax warpgroup holds 32 columns of either half; in
+// dK/dV its values replace the scores at the place they came from, in dQ they lie packed.
+template <bool kPacked>
+__device__ __forceinline__ void issue_acc_half(uint32_t d_tmem, uint32_t a_tmem, uint32_t y_lo, int half,
+                                               uint32_t accumulate) {
+  constexpr uint32_t idesc = idesc_bf16_f32(kTile, kHeadDim, 0, 1);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int kk = half * 4 + q;
+    mma_ts_lo(d_tmem, a_tmem + (kPacked ? kk * 8 : (kk >> 1) * 32 + (kk & 1) * 8), y_lo + ((kk * 16 * 128) >> 4),
+              kDescHiSw128, idesc, accumulate | (kk > 0 ? 1u : 0u));
+  }
+}
+
+template <bool kPacked>
+__device__ __forceinline__ void issue_acc(uint32_t d_tmem, uint32_t a_tmem, uint32_t y_lo, uint32_t accumulate) {
+  issue_acc_half<kPacked>(d_tmem, a_tmem, y_lo, 0, accumulate);
+  issue_acc_half<kPacked>(d_tmem, a_tmem, y_lo, 1, accumulate);
 }
 
 // 2^x for pair number `i` of a chunk: kEmu of every 8 pairs on the FMA pipe (results below
@@ -253,6 +324,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__ CUtensorMap tm_x2,
                     const __grid_constant__ CUtensorMap tm_y1, const __grid_constant__ CUtensorMap tm_y2,
                     const __grid_constant__ BwdParams p) {
+  using Sm = Smem<kDq>;
+  constexpr int kY1 = Sm::kY1;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_addr(smem);
   const int warp = threadIdx.x >> 5;
@@ -298,27 +371,48 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp < kEpiWarp) {
     regs_increase<kBwdRegsSoftmax>();
     // ------------------------------------------------------------ softmax
+    // Each warpgroup takes 32 columns of either half of the tile: [32 wg, 32 wg + 32) and
+    // 64 further on.
     const int wg = warp >> 2;
     const int wq = warp & 3;
     const int row = threadIdx.x & 127;
-    const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 64;
+    const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 32;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     bool ok = true;
     uint32_t n = 0;
     float neg_lse = 0.f, neg_delta = 0.f;
     Tiles<kDq> it(p);
-    while (it.next()) {
+    // The barrier rounds of a tile from round `from` on, blocking: after an abort a warp
+    // keeps its place in the issuer's schedule with these.
+    auto keep_rounds = [&](int from) {
+      __syncwarp();
+      if (kDq) {
+        if (from < 1) named_bar_sync(bar_tile(kRoundT1Read, n), kTileThreads);
+        if (from < 2) named_bar_sync(bar_tile(kRoundT2Read, n), kTileThreads);
+      } else if (from < 1) {
+        named_bar_sync(bar_tile(kRoundP0, n), kHalfThreads);
+        named_bar_sync(bar_tile(kRoundP1, n), kTileThreads);
+      }
+      named_bar_sync(bar_tile(kRoundDs, n), kDsThreads<kDq>);
+    };
+    // dQ: the statistics of this row in the item after the current one, loaded an item ahead.
+    Items<kDq> ahead(p);
+    float next_lse = 0.f, next_delta = 0.f;
+    auto load_stats = [&]() {
+      if (!ahead.next_busy()) return;
+      const float* st = p.stats + (static_cast<long long>(ahead.head) * p.nq + ahead.tile) * (2 * kTile);
+      next_lse = __ldg(st + row);
+      next_delta = __ldg(st + kTile + row);
+    };
+    if (kDq) load_stats();
+    for (; it.next(); ++n) {
       if (!ok) {
-        // After an abort: keep this warp's place in the issuer's barrier rounds.
-        __syncwarp();
-        if (!kDq) named_bar_sync(kBarP, kSoftmaxThreads + 32);
-        named_bar_sync(kBarDs, kSoftmaxThreads + 32);
+        keep_rounds(0);
         continue;
       }
-      const uint32_t tT1 = tBase + ((kDq && (n & 1)) ? kColAcc2 : kColT1);
-      const uint32_t tT2 = tBase + kColT2;
+      const uint32_t tT1 = tBase + kColT1, tT2 = tBase + kColT2;
       // Columns [lo, hi) of this tile are visible to this row; mask_tile: some row of the
-      // warp sees fewer than this warpgroup's 64.
+      // warp does not see all of this warpgroup's columns.
       int lo = 0, hi = kTile;
       bool mask_tile;
       if (kDq) {
@@ -330,110 +424,131 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           hi = min(hi, q + p.offset - key0 + 1);
           hi_warp = min(hi_warp, q - lane + p.offset - key0 + 1);
         }
-        mask_tile = hi_warp < wg * 64 + 64;
+        mask_tile = hi_warp < kTile;
         if (it.first) {
-          const float* st = p.stats + (static_cast<long long>(it.items.head) * p.nq + it.items.tile) * (2 * kTile);
-          neg_lse = __ldg(st + row);
-          neg_delta = __ldg(st + kTile + row);
+          neg_lse = next_lse;
+          neg_delta = next_delta;
+          load_stats();
         }
       } else {
         const int key = it.items.tile * kTile + row;
         lo = p.causal ? key - p.offset - it.t * kTile : 0;
-        mask_tile = p.causal && (key - lane + 31 - p.offset - it.t * kTile) > wg * 64;
+        mask_tile = p.causal && key - lane + 31 - p.offset - it.t * kTile > 0;
       }
-      const int t1_bar = kDq ? B_T1_FULL + static_cast<int>(n & 1) : B_T1_FULL;
-      ok = wait_phase(bar(t1_bar), kDq ? (n >> 1) & 1 : n & 1, watch);
-      if (!kDq) ok = ok && wait_phase(bar(B_STAT + static_cast<int>(n & 1)), (n >> 1) & 1, watch);
+      const uint32_t phase = (n >> 1) & 1;
+      ok = wait_phase(bar(B_T1_FULL + static_cast<int>(n & 1)), phase, watch);
+      if (!kDq) ok = ok && wait_phase(bar(B_STAT + static_cast<int>(n & 1)), phase, watch);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
-        if (!kDq) named_bar_sync(kBarP, kSoftmaxThreads + 32);
-        named_bar_sync(kBarDs, kSoftmaxThreads + 32);
-        ++n;
+        keep_rounds(0);
         continue;
       }
       tc_fence_after();
-      // P for this warpgroup's 64 columns: fp32 pairs kept for dS, bf16 to TMEM (dK/dV only).
+      AVO_TRACE_HOOK(wg, n, 0);
+      // P: fp32 pairs kept for dS, bf16 to TMEM (dK/dV only) a half at a time, so that dV's
+      // first MMAs overlap the second half's exponentials.
       uint64_t pr[32];
       {
         uint32_t s[2][32];
         tmem_ld32(tT1, s[0]);
-        tmem_ld32(tT1 + 32, s[1]);
+        tmem_ld32(tT1 + 64, s[1]);
+        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + wg * 128;
+        const uint64_t neg2 = f2_pack(neg_lse, neg_lse);
         tmem_wait_ld(s[0]);
         tmem_wait_ld(s[1]);
-        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + wg * 256;
-        const uint64_t neg2 = f2_pack(neg_lse, neg_lse);
+        if (kDq) {
+          // S_{n+1} may overwrite T1.
+          tc_fence_before();
+          __syncwarp();
+          named_bar_arrive(bar_tile(kRoundT1Read, n), kTileThreads);
+        }
+        AVO_TRACE_HOOK(wg, n, 1);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             uint64_t la = neg2, lb = neg2;
-            if (!kDq) lds_f2x2(stat + (c * 32 + e * 2) * 4, la, lb);
+            if (!kDq) lds_f2x2(stat + (c * 64 + e * 2) * 4, la, lb);
             pr[c * 16 + e] =
                 exp2_pair<2>(e, f2_fma(f2_pack(u2f(s[c][2 * e]), u2f(s[c][2 * e + 1])), scale2, la));
             pr[c * 16 + e + 1] =
                 exp2_pair<2>(e + 1, f2_fma(f2_pack(u2f(s[c][2 * e + 2]), u2f(s[c][2 * e + 3])), scale2, lb));
           }
+          if (mask_tile) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, b;
+              f2_unpack(pr[c * 16 + i], a, b);
+              const int col = c * 64 + wg * 32 + 2 * i;
+              a = (col >= lo && col < hi) ? a : 0.f;
+              b = (col + 1 >= lo && col + 1 < hi) ? b : 0.f;
+              pr[c * 16 + i] = f2_pack(a, b);
+            }
+          }
+          if (!kDq) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack_pair(pr[c * 16 + i]);
+            tmem_st16(tT1 + c * 64, w);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            named_bar_arrive(bar_tile(c == 0 ? kRoundP0 : kRoundP1, n), c == 0 ? kHalfThreads : kTileThreads);
+          }
         }
       }
-      if (mask_tile) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float a, b;
-          f2_unpack(pr[i], a, b);
-          const int col = wg * 64 + 2 * i;
-          a = (col >= lo && col < hi) ? a : 0.f;
-          b = (col + 1 >= lo && col + 1 < hi) ? b : 0.f;
-          pr[i] = f2_pack(a, b);
-        }
-      }
-      if (!kDq) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack_pair(pr[c * 16 + i]);
-          tmem_st16(tT1 + c * 16, w);
-        }
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        named_bar_arrive(kBarP, kSoftmaxThreads + 32);
-      }
-      ok = __all_sync(0xffffffffu, wait_phase(bar(B_T2_FULL), n & 1, watch));
+      AVO_TRACE_HOOK(wg, n, 2);
+      ok = __all_sync(0xffffffffu, wait_phase(bar(B_T2_FULL + static_cast<int>(n & 1)), phase, watch));
       if (!ok) {
-        named_bar_sync(kBarDs, kSoftmaxThreads + 32);
-        ++n;
+        keep_rounds(1);
         continue;
       }
       tc_fence_after();
+      AVO_TRACE_HOOK(wg, n, 3);
       {
         uint32_t d[2][32];
         tmem_ld32(tT2, d[0]);
-        tmem_ld32(tT2 + 32, d[1]);
+        tmem_ld32(tT2 + 64, d[1]);
         tmem_wait_ld(d[0]);
         tmem_wait_ld(d[1]);
-        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + kTile * 4 + wg * 256;
+        if (kDq) {
+          // dP_{n+1} may overwrite T2 while dS_n is computed.
+          tc_fence_before();
+          __syncwarp();
+          named_bar_arrive(bar_tile(kRoundT2Read, n), kTileThreads);
+        }
+        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + kTile * 4 + wg * 128;
         const uint64_t neg2 = f2_pack(neg_delta, neg_delta);
-        const uint32_t tDs = kDq ? tT1 : tT2;
+        const uint32_t tDs = kDq ? tBase - wg * 16 + kColDs : tT2;
+        if (kDq && n > 0) {
+          // dQ_{n-1} has read the previous dS.
+          const uint32_t u = n - 1;
+          ok = __all_sync(0xffffffffu, wait_phase(bar(B_Y1_EMPTY + static_cast<int>(u % kY1)), (u / kY1) & 1, watch));
+          if (!ok) {
+            keep_rounds(2);
+            continue;
+          }
+          tc_fence_after();
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             uint64_t la = neg2, lb = neg2;
-            if (!kDq) lds_f2x2(stat + (c * 32 + e * 2) * 4, la, lb);
+            if (!kDq) lds_f2x2(stat + (c * 64 + e * 2) * 4, la, lb);
             w[e] = pack_pair(f2_mul(pr[c * 16 + e], f2_add(f2_pack(u2f(d[c][2 * e]), u2f(d[c][2 * e + 1])), la)));
             w[e + 1] = pack_pair(
                 f2_mul(pr[c * 16 + e + 1], f2_add(f2_pack(u2f(d[c][2 * e + 2]), u2f(d[c][2 * e + 3])), lb)));
           }
-          tmem_st16(tDs + c * 16, w);
+          tmem_st16(tDs + c * (kDq ? 32 : 64), w);
         }
       }
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      named_bar_arrive(kBarDs, kSoftmaxThreads + 32);
-      ++n;
+      named_bar_arrive(bar_tile(kRoundDs, n), kDsThreads<kDq>);
+      AVO_TRACE_HOOK(wg, n, 4);
     }
   } else if (warp < kProducerWarp) {
     regs_decrease<kBwdRegsEpi>();
@@ -442,9 +557,56 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int rows = kDq ? p.seq_q : p.seq_kv;
     bool ok = true;
-    uint32_t done = 0;  // items with tiles so far
+    uint32_t done = 0;   // items with tiles so far
+    // dQ: this thread's row of Q of the next item with tiles, loaded an item ahead.
+    Items<kDq> ahead(p);
+    uint32_t xq[64];
+    bool have_x = false;
+    auto load_x = [&]() {
+      have_x = ahead.next_busy();
+      const int r = ahead.tile * kTile + row;
+      if (have_x && r < rows) {
+        const uint4* src = static_cast<const uint4*>(p.x1) + (static_cast<long long>(ahead.head) * rows + r) * 16;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint4 v = __ldg(src + i);
+          xq[4 * i] = v.x;
+          xq[4 * i + 1] = v.y;
+          xq[4 * i + 2] = v.z;
+          xq[4 * i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) xq[i] = 0u;
+      }
+    };
+    uint32_t x_signals = 0, acc_signals = 0;
+    auto store_x = [&]() {
+      const uint32_t t = tmem + lane_off + kColX1;
+#pragma unroll
+      for (int i = 0; i < 64; i += 8)
+        tmem_st8(t + i, xq[i], xq[i + 1], xq[i + 2], xq[i + 3], xq[i + 4], xq[i + 5], xq[i + 6], xq[i + 7]);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      named_bar_arrive(bar_x1(x_signals++), kEpiThreads);
+    };
+    if (kDq) {
+      load_x();
+      if (have_x) store_x();
+    }
     Items<kDq> it(p);
-    while (it.next()) {
+    while (ok && it.next()) {
+      if (kDq && it.n > 0) {
+        load_x();
+        if (have_x) {
+          // Q may be replaced once this item's last S is done with it.
+          ok = wait_item(bar(B_X1_DONE), done & 1, it.n, watch, lane);
+          if (!ok) break;
+          tc_fence_after();
+          store_x();
+        }
+      }
       const int r = it.tile * kTile + row;
       const bool write = r < rows;
       const long long at = (static_cast<long long>(it.head) * rows + r) * kHeadDim;
@@ -454,14 +616,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __nv_bfloat16* const dst = static_cast<__nv_bfloat16*>(a == 1 ? p.g1 : p.g2) + at;
         const float f = a == 1 ? p.scale : 1.f;
         const uint32_t acc = tmem + lane_off + (a == 1 ? kColAcc1 : kColAcc2);
-        if (it.n > 0 && ok) {
-          ok = __all_sync(0xffffffffu, wait_phase(bar(a == 1 ? B_ACC1 : B_ACC2), done & 1, watch));
+        if (it.n > 0) {
+          ok = wait_item(bar(a == 1 ? B_ACC1 : B_ACC2), done & 1, it.n, watch, lane);
+          if (!ok) break;
           tc_fence_after();
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          if (it.n > 0 && ok) {
+          if (it.n > 0) {
             tmem_ld32(acc + c * 32, o);
             tmem_wait_ld(o);
           } else {
@@ -472,12 +635,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             // Read out: the next item may overwrite it.
             tc_fence_before();
             __syncwarp();
-            if (ok)
-              named_bar_arrive(a == 1 ? kBarAcc1 : kBarAcc2, 128 + 32);
-            else
-              named_bar_sync(a == 1 ? kBarAcc1 : kBarAcc2, 128 + 32);
+            named_bar_arrive(a == 1 ? bar_acc1(done) : bar_acc2(done), kEpiThreads);
+            ++acc_signals;
           }
-          if (write && ok) {
+          if (write) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               uint32_t w[8];
@@ -491,6 +652,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (it.n > 0) ++done;
     }
+    if (!ok) {
+      // After an abort: the signals not given yet, as blocking syncs in the issuer's order.
+      __syncwarp();
+      uint32_t x_seen = 0, acc_seen = 0, item = 0;
+      auto x_round = [&]() {
+        if (x_seen >= x_signals) named_bar_sync(bar_x1(x_seen), kEpiThreads);
+        ++x_seen;
+      };
+      auto acc_round = [&](uint32_t i) {
+        if (!kDq && acc_seen++ >= acc_signals) named_bar_sync(bar_acc2(i), kEpiThreads);
+        if (acc_seen++ >= acc_signals) named_bar_sync(bar_acc1(i), kEpiThreads);
+      };
+      Items<kDq> all(p), after(p);
+      bool more = after.next_busy();
+      if (kDq && more) x_round();
+      for (; all.next_busy(); ++item) {
+        more = after.next_busy();
+        if (kDq && more && all.n == 1) x_round();
+        if (item > 0) acc_round(item - 1);
+        if (kDq && more && all.n > 1) x_round();
+        if (!more) acc_round(item);
+      }
+    }
   } else if (warp == kProducerWarp) {
     regs_decrease<kBwdRegsOther>();
     // ------------------------------------------------------------ TMA producer
@@ -502,43 +686,71 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tma_load_3d(sbase + off, tm, bar(b), 0, r0, head, pol);
         tma_load_3d(sbase + off + kHalfBytes, tm, bar(b), 64, r0, head, pol);
       };
-      // Waits until a buffer's last user is done and its previous copy has landed (the
-      // latter is implied unless the CTA aborted): at most one copy per buffer in flight.
-      auto reuse = [&](int empty, int full, uint32_t parity) {
-        return wait_phase(bar(empty), parity, watch) && wait_phase(bar(full), parity, watch) && !*abort_flag;
+      // A buffer may be loaded again once its last user is done and its previous copy has
+      // landed (implied unless the CTA aborted): at most one copy per buffer is in flight.
+      auto reuse_after = [&](int done, uint32_t done_parity, int full, uint32_t full_parity) {
+        return wait_phase(bar(done), done_parity, watch) && wait_phase(bar(full), full_parity, watch) && !*abort_flag;
       };
-      int n = 0, items = 0, n2 = 0, nx2 = 0, nst = 0, skipped = -1;
+      // ... done as tile u's T1 or T2 commit implies.
+      auto reuse = [&](int commit, int u, int full, uint32_t full_parity) {
+        return reuse_after(commit + (u & 1), (u >> 1) & 1, full, full_parity);
+      };
+      int n = 0, n2 = 0, nx1 = 0, nx2 = 0, nst = 0, skipped = -1;
+      // The stationary tiles of the next item, and its first streamed ones, are brought to L2
+      // while this item runs: their loads start only when its last tiles are done with the
+      // buffers.
+      Items<kDq> ahead(p);
+      ahead.next_busy();
+      auto prefetch = [&](const CUtensorMap* tm, int r0, int head) {
+        tma_prefetch_3d(tm, 0, r0, head);
+        tma_prefetch_3d(tm, 64, r0, head);
+      };
       Tiles<kDq> it(p);
       while (it.next()) {
+        if (it.first && ahead.next_busy()) {
+          const int y_head = kDq ? ahead.head / p.group : ahead.head * p.group;
+          if (!kDq) prefetch(&tm_x1, ahead.tile * kTile, ahead.head);
+          prefetch(&tm_x2, ahead.tile * kTile, ahead.head);
+          prefetch(&tm_y1, ahead.t0 * kTile, y_head);
+          prefetch(&tm_y2, ahead.t0 * kTile, y_head);
+        }
         const int s1 = n % kY1, s2 = n % kY2;
-        if (n >= kY1 && !reuse(B_Y1_EMPTY + s1, B_Y1_FULL + s1, (n / kY1 - 1) & 1)) break;
+        // Y1's last user is its tile's last MMA: dQ, or dK, which precedes the next tile's T2.
+        if (n >= kY1) {
+          const uint32_t before = (n / kY1 - 1) & 1;
+          if (!(kDq ? reuse_after(B_Y1_EMPTY + s1, before, B_Y1_FULL + s1, before)
+                    : reuse(B_T2_FULL, n - 2, B_Y1_FULL + s1, before)))
+            break;
+        }
         if (*abort_flag) break;
         if (n == p.test_skip_load) skipped = n;  // test hook: this copy never arrives
-        if (n != skipped) load(kSmY1 + s1 * kTileBytes, &tm_y1, B_Y1_FULL + s1, it.t * kTile, it.y_head, pol_y);
+        if (n != skipped) load(Sm::kY1At + s1 * kTileBytes, &tm_y1, B_Y1_FULL + s1, it.t * kTile, it.y_head, pol_y);
         ++n;
-        if (it.first) {
-          if (items > 0 && !reuse(B_X1_EMPTY, B_X1_FULL, (items - 1) & 1)) break;
-          load(kSmX1, &tm_x1, B_X1_FULL, it.items.tile * kTile, it.items.head, pol_x);
-          ++items;
+        const int last = n - 2;  // the previous tile
+        if (!kDq && it.first) {
+          // X1 was read last by the previous tile's T1, X2 by its T2.
+          if (nx1 > 0 && !reuse(B_T1_FULL, last, B_X1_FULL, (nx1 - 1) & 1)) break;
+          load(Sm::kX1, &tm_x1, B_X1_FULL, it.items.tile * kTile, it.items.head, pol_x);
+          ++nx1;
         }
-        if (n2 >= kY2 && !reuse(B_Y2_EMPTY + s2, B_Y2_FULL + s2, (n2 / kY2 - 1) & 1)) break;
-        load(kSmY2 + s2 * kTileBytes, &tm_y2, B_Y2_FULL + s2, it.t * kTile, it.y_head, pol_y);
+        // Y2's last user is dV, before T1 of the next tile (dK/dV), or T2 itself (dQ).
+        if (n2 >= kY2 && !reuse(kDq ? B_T2_FULL : B_T1_FULL, kDq ? last - 1 : last, B_Y2_FULL + s2, (n2 / kY2 - 1) & 1))
+          break;
+        load(Sm::kY2At + s2 * kTileBytes, &tm_y2, B_Y2_FULL + s2, it.t * kTile, it.y_head, pol_y);
         ++n2;
         if (it.first) {
-          if (nx2 > 0 && !reuse(B_X2_EMPTY, B_X2_FULL, (nx2 - 1) & 1)) break;
-          load(kSmX2, &tm_x2, B_X2_FULL, it.items.tile * kTile, it.items.head, pol_x);
+          if (nx2 > 0 && !reuse(B_T2_FULL, last, B_X2_FULL, (nx2 - 1) & 1)) break;
+          load(Sm::kX2, &tm_x2, B_X2_FULL, it.items.tile * kTile, it.items.head, pol_x);
           ++nx2;
         }
         if (!kDq) {
-          // The slot's last readers published dS of tile nst - 2 before that tile's dK MMAs,
-          // whose completion empties its Y1 slot.
-          const int u = nst - 2;
-          if (u >= 0 && !(wait_phase(bar(B_Y1_EMPTY + u % kY1), (u / kY1) & 1, watch) &&
-                          wait_phase(bar(B_STAT + (u & 1)), (u >> 1) & 1, watch) && !*abort_flag))
-            break;
+          // The slot's last readers published dS of tile nst - 2 before that tile's dK, which
+          // precedes T2 of tile nst - 1.
+          const int slot = nst & 1;
+          if (nst >= 2 && !reuse(B_T2_FULL, nst - 1, B_STAT + slot, ((nst >> 1) - 1) & 1)) break;
           const float* src = p.stats + (static_cast<long long>(it.y_head) * p.nq + it.t) * (2 * kTile);
-          mbar_arrive_expect_tx(bar(B_STAT + (nst & 1)), kStatBytes);
-          bulk_load(sbase + kSmStat + (nst & 1) * kStatBytes, src, kStatBytes, bar(B_STAT + (nst & 1)));
+          mbar_arrive_expect_tx(bar(B_STAT + slot), kStatBytes);
+          bulk_load(sbase + kSmStat + slot * kStatBytes, src, kStatBytes, bar(B_STAT + slot));
           ++nst;
         }
       }
@@ -548,7 +760,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (u != skipped) drain_phase(bar(B_Y1_FULL + u % kY1), (u / kY1) & 1, watch);
         for (int u = max(0, n2 - kY2); u < n2; ++u) drain_phase(bar(B_Y2_FULL + u % kY2), (u / kY2) & 1, watch);
         for (int u = max(0, nst - 2); u < nst; ++u) drain_phase(bar(B_STAT + (u & 1)), (u >> 1) & 1, watch);
-        if (items > 0) drain_phase(bar(B_X1_FULL), (items - 1) & 1, watch);
+        if (nx1 > 0) drain_phase(bar(B_X1_FULL), (nx1 - 1) & 1, watch);
         if (nx2 > 0) drain_phase(bar(B_X2_FULL), (nx2 - 1) & 1, watch);
       }
     }
@@ -556,13 +768,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   } else if (warp == kIssuerWarp) {
     regs_decrease<kBwdRegsOther>();
     // ------------------------------------------------------------ MMA issuer
-    const bool leader = lane == 0;
+    // The issuing lane is chosen by elect.sync: with `lane == 0` the compiler moves every
+    // operand of every MMA to uniform registers one lane at a time, and issuing became the
+    // limit (measured on B200, B1 H16 S4096: 3324 and 2731 cycles per tile pair of the two
+    // passes, 2814 and 2104 with elect.sync).
+    const bool leader = elect_one();
     const uint32_t tT1 = tmem + kColT1, tT2 = tmem + kColT2, tA1 = tmem + kColAcc1, tA2 = tmem + kColAcc2;
-    const uint32_t x1 = smem_desc_lo(sbase + kSmX1, 16), x2 = smem_desc_lo(sbase + kSmX2, 16);
+    const uint32_t tDs = tmem + kColDs, tX1 = tmem + kColX1;
+    const uint32_t x1 = smem_desc_lo(sbase + Sm::kX1, 16), x2 = smem_desc_lo(sbase + Sm::kX2, 16);
     // Streamed tiles as the N x K operand of T1 and T2, and as the K x N operand of the
     // accumulating MMAs.
-    const uint32_t y1 = smem_desc_lo(sbase + kSmY1, 16), y1t = smem_desc_lo(sbase + kSmY1, kHalfBytes);
-    const uint32_t y2 = smem_desc_lo(sbase + kSmY2, 16), y2t = smem_desc_lo(sbase + kSmY2, kHalfBytes);
+    const uint32_t y1 = smem_desc_lo(sbase + Sm::kY1At, 16), y1t = smem_desc_lo(sbase + Sm::kY1At, kHalfBytes);
+    const uint32_t y2 = smem_desc_lo(sbase + Sm::kY2At, 16), y2t = smem_desc_lo(sbase + Sm::kY2At, kHalfBytes);
     constexpr uint32_t kSlot = kTileBytes >> 4;
     auto sync_on = [&](uint32_t id, uint32_t threads) {
       __syncwarp();
@@ -571,140 +788,69 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     };
     Tiles<kDq> it(p);
     uint32_t items = 0;
-    if constexpr (!kDq) {
-      bool have = it.next();
-      int s1 = 0, s2 = 0;  // slots of the current tile
-      if (have) {
-        sync_on(kBarLoaded, 64);
+    auto issue_t1 = [&](int slot, int parity) {
+      if constexpr (kDq)
+        issue_xy_tmem(tT1, tX1, y1 + slot * kSlot);
+      else
+        issue_xy(tT1, x1, y1 + slot * kSlot);
+      mma_commit(bar(B_T1_FULL + parity));
+      if (kDq && it.last) mma_commit(bar(B_X1_DONE));
+    };
+    auto issue_t2 = [&](int parity) {  // the parity is also the Y2 slot
+      issue_xy(tT2, x2, y2 + parity * kSlot);
+      mma_commit(bar(B_T2_FULL + parity));
+    };
+    bool have = it.next();
+    if (have) {
+      sync_on(kBarLoaded, 64);
+      if (kDq) sync_on(bar_x1(0), kEpiThreads);
+      if (leader) issue_t1(0, 0);
+      sync_on(kBarLoaded, 64);
+      if (leader) issue_t2(0);
+    }
+    int s1 = 0, par = 0;  // Y1 slot of the current tile; its parity
+    while (have) {
+      const bool first = it.first, last = it.last;
+      have = it.next();  // now: the tile after the current one
+      const int n1 = s1 == kY1 - 1 ? 0 : s1 + 1, other = par ^ 1;
+      if constexpr (!kDq) {
+        if (first && items > 0) sync_on(bar_acc2(items - 1), kEpiThreads);
+        sync_on(bar_tile(kRoundP0, par), kHalfThreads);
+        if (leader) issue_acc_half<false>(tA2, tT1, y2t + par * kSlot, 0, first ? 0u : 1u);
+        sync_on(bar_tile(kRoundP1, par), kTileThreads);
         if (leader) {
-          issue_xy(tT1, x1, y1);
-          mma_commit(bar(B_T1_FULL));
-          if (it.last) mma_commit(bar(B_X1_EMPTY));
-        }
-        sync_on(kBarLoaded, 64);
-        if (leader) {
-          issue_xy(tT2, x2, y2);
-          mma_commit(bar(B_T2_FULL));
-          if (it.last) mma_commit(bar(B_X2_EMPTY));
-        }
-      }
-      while (have) {
-        const bool first = it.first, last = it.last;
-        const bool more = it.next();
-        const bool next_last = more && it.last;
-        const int n1 = s1 == kY1 - 1 ? 0 : s1 + 1, n2 = s2 ^ 1;
-        if (first && items > 0) sync_on(kBarAcc2, 128 + 32);
-        sync_on(kBarP, kSoftmaxThreads + 32);
-        if (leader) {
-          issue_acc(tA2, tT1, y2t + s2 * kSlot, first ? 0u : 1u);
-          mma_commit(bar(B_Y2_EMPTY + s2));
+          issue_acc_half<false>(tA2, tT1, y2t + par * kSlot, 1, 1u);
           if (last) mma_commit(bar(B_ACC2));
+          if (have) issue_t1(n1, other);
         }
-        if (more) {
-          sync_on(kBarLoaded, 64);
-          if (leader) {
-            issue_xy(tT1, x1, y1 + n1 * kSlot);
-            mma_commit(bar(B_T1_FULL));
-            if (next_last) mma_commit(bar(B_X1_EMPTY));
-          }
-        }
-        if (first && items > 0) sync_on(kBarAcc1, 128 + 32);
-        sync_on(kBarDs, kSoftmaxThreads + 32);
+        if (first && items > 0) sync_on(bar_acc1(items - 1), kEpiThreads);
+        sync_on(bar_tile(kRoundDs, par), kTileThreads);
         if (leader) {
-          issue_acc(tA1, tT2, y1t + s1 * kSlot, first ? 0u : 1u);
+          issue_acc<false>(tA1, tT2, y1t + s1 * kSlot, first ? 0u : 1u);
+          if (last) mma_commit(bar(B_ACC1));
+          if (have) issue_t2(other);
+        }
+      } else {
+        sync_on(bar_tile(kRoundT1Read, par), kTileThreads);
+        if (have && it.first) sync_on(bar_x1(items + (first ? 1 : 0)), kEpiThreads);
+        if (leader && have) issue_t1(n1, other);
+        sync_on(bar_tile(kRoundT2Read, par), kTileThreads);
+        if (leader && have) issue_t2(other);
+        if (first && items > 0) sync_on(bar_acc1(items - 1), kEpiThreads);
+        sync_on(bar_tile(kRoundDs, par), kHalfThreads);
+        if (leader) {
+          issue_acc<true>(tA1, tDs, y1t + s1 * kSlot, first ? 0u : 1u);
           mma_commit(bar(B_Y1_EMPTY + s1));
           if (last) mma_commit(bar(B_ACC1));
         }
-        if (more) {
-          sync_on(kBarLoaded, 64);
-          if (leader) {
-            issue_xy(tT2, x2, y2 + n2 * kSlot);
-            mma_commit(bar(B_T2_FULL));
-            if (next_last) mma_commit(bar(B_X2_EMPTY));
-          }
-        }
-        if (first) ++items;
-        s1 = n1;
-        s2 = n2;
-        have = more;
       }
-      if (items > 0) {
-        sync_on(kBarAcc2, 128 + 32);
-        sync_on(kBarAcc1, 128 + 32);
-      }
-    } else {
-      // S runs two tiles ahead (T1 | acc2 columns are its two buffers), dP one.
-      bool f0 = false, l0 = false, f1 = false, l1 = false;
-      bool have = it.next(), have1 = false;
-      if (have) {
-        f0 = it.first;
-        l0 = it.last;
-        sync_on(kBarLoaded, 64);
-        if (leader) {
-          issue_xy(tT1, x1, y1);
-          mma_commit(bar(B_T1_FULL));
-          if (l0) mma_commit(bar(B_X1_EMPTY));
-        }
-        sync_on(kBarLoaded, 64);
-        if (leader) {
-          issue_xy(tT2, x2, y2);
-          mma_commit(bar(B_T2_FULL));
-          mma_commit(bar(B_Y2_EMPTY));
-          if (l0) mma_commit(bar(B_X2_EMPTY));
-        }
-        have1 = it.next();
-        f1 = it.first;
-        l1 = it.last;
-        if (have1) {
-          sync_on(kBarLoaded, 64);
-          if (leader) {
-            issue_xy(tA2, x1, y1 + kSlot);
-            mma_commit(bar(B_T1_FULL + 1));
-            if (l1) mma_commit(bar(B_X1_EMPTY));
-          }
-        }
-      }
-      int s1 = 0, par = 0;
-      while (have) {
-        const bool have2 = have1 && it.next();
-        const bool f2 = it.first, l2 = it.last;
-        const int s1_2 = s1 == 0 ? 2 : s1 - 1;  // slot of tile n + 2
-        const uint32_t tS = par ? tA2 : tT1;
-        sync_on(kBarDs, kSoftmaxThreads + 32);
-        if (have1) {
-          sync_on(kBarLoaded, 64);
-          if (leader) {
-            issue_xy(tT2, x2, y2 + (par ^ 1) * kSlot);
-            mma_commit(bar(B_T2_FULL));
-            mma_commit(bar(B_Y2_EMPTY + (par ^ 1)));
-            if (l1) mma_commit(bar(B_X2_EMPTY));
-          }
-        }
-        if (f0 && items > 0) sync_on(kBarAcc1, 128 + 32);
-        if (leader) {
-          issue_acc(tA1, tS, y1t + s1 * kSlot, f0 ? 0u : 1u);
-          mma_commit(bar(B_Y1_EMPTY + s1));
-          if (l0) mma_commit(bar(B_ACC1));
-        }
-        if (have2) {
-          sync_on(kBarLoaded, 64);
-          if (leader) {
-            issue_xy(tS, x1, y1 + s1_2 * kSlot);
-            mma_commit(bar(B_T1_FULL + par));
-            if (l2) mma_commit(bar(B_X1_EMPTY));
-          }
-        }
-        if (f0) ++items;
-        f0 = f1;
-        l0 = l1;
-        f1 = f2;
-        l1 = l2;
-        have = have1;
-        have1 = have2;
-        s1 = s1 == kY1 - 1 ? 0 : s1 + 1;
-        par ^= 1;
-      }
-      if (items > 0) sync_on(kBarAcc1, 128 + 32);
+      if (first) ++items;
+      s1 = n1;
+      par = other;
+    }
+    if (items > 0) {
+      if (!kDq) sync_on(bar_acc2(items - 1), kEpiThreads);
+      sync_on(bar_acc1(items - 1), kEpiThreads);
     }
     __syncwarp();
     if (leader && items > 0) {
@@ -716,25 +862,46 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   } else if (warp == kWaiterWarp) {
     regs_decrease<kBwdRegsOther>();
     // ------------------------------------------------------------ waiter
-    // The loads' mbarrier waits in the issuer's order: X1 and Y1 of a tile for T1, X2 and Y2
-    // for T2.  After an abort the waits return at once and only the rounds are kept.
-    int n = 0, items = 0;
+    // The loads' mbarrier waits in the issuer's order (X1 and Y1 of a tile for T1, X2 and Y2
+    // for T2); then its rounds on the barriers whose release lets the issuer use them.  After
+    // an abort the waits return at once and only the rounds are kept.
+    int n1 = 0, n2 = 0, x1 = 0, x2 = 0;
+    Tiles<kDq> a(p), c(p);  // tiles whose T1 / T2 operands are next
+    auto t1_loaded = [&]() {
+      if (!a.next()) return;
+      if (lane == 0) {
+        if (!kDq && a.first) wait_phase(bar(B_X1_FULL), x1 & 1, watch);
+        wait_phase(bar(B_Y1_FULL + n1 % kY1), (n1 / kY1) & 1, watch);
+      }
+      if (a.first) ++x1;
+      ++n1;
+    };
+    auto t2_loaded = [&]() {
+      if (!c.next()) return;
+      if (lane == 0) {
+        if (c.first) wait_phase(bar(B_X2_FULL), x2 & 1, watch);
+        wait_phase(bar(B_Y2_FULL + n2 % kY2), (n2 / kY2) & 1, watch);
+      }
+      if (c.first) ++x2;
+      ++n2;
+    };
+    auto round = [&](uint32_t id, uint32_t threads) {
+      __syncwarp();
+      named_bar_sync(id, threads);
+    };
     Tiles<kDq> it(p);
-    while (it.next()) {
-      if (lane == 0) {
-        if (it.first) wait_phase(bar(B_X1_FULL), items & 1, watch);
-        wait_phase(bar(B_Y1_FULL + n % kY1), (n / kY1) & 1, watch);
-      }
-      __syncwarp();
-      named_bar_sync(kBarLoaded, 64);
-      if (lane == 0) {
-        if (it.first) wait_phase(bar(B_X2_FULL), items & 1, watch);
-        wait_phase(bar(B_Y2_FULL + n % kY2), (n / kY2) & 1, watch);
-      }
-      __syncwarp();
-      named_bar_sync(kBarLoaded, 64);
-      if (it.first) ++items;
-      ++n;
+    bool have = it.next();
+    if (have) {
+      t1_loaded();
+      round(kBarLoaded, 64);
+      t2_loaded();
+      round(kBarLoaded, 64);
+    }
+    for (uint32_t n = 0; have; have = it.next(), ++n) {
+      t1_loaded();
+      round(bar_tile(kDq ? kRoundT1Read : kRoundP1, n), kTileThreads);
+      t2_loaded();
+      round(bar_tile(kDq ? kRoundT2Read : kRoundDs, n), kTileThreads);
     }
   } else {
     regs_decrease<kBwdRegsOther>();  // warp 15 completes the warpgroup
