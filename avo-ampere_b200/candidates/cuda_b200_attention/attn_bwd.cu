@@ -129,6 +129,13 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.test_skip_load = host::skip_load();
 
+  const long long kv_items = static_cast<long long>(kv_all) * p.nkv, q_items = static_cast<long long>(q_heads) * p.nq;
+  // Both passes at once where the dK/dV grid leaves multiprocessors idle from the start.
+  // Measured on B200, at once against one after the other: B1 H4 S512 14.1 / 22.9 us, B1 H16
+  // Hkv2 Q777 KV5003 137 / 144 us; but B1 H16 S4096 493 / 417 us: both passes slow down while
+  // they share the chip.
+  p.overlap = kv_items < sms ? 1 : 0;
+
   const long long rows = static_cast<long long>(q_heads) * p.nq * kTile;
   const long long blocks = rows / 16;
   if (blocks > INT_MAX) return AVO_B200_EINVAL;
@@ -136,7 +143,6 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
                           static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse,
                           static_cast<float*>(workspace), rows, seq_q, p.nq))
     return AVO_B200_ELAUNCH;
-  const long long kv_items = static_cast<long long>(kv_all) * p.nkv, q_items = static_cast<long long>(q_heads) * p.nq;
   p.g1 = dk;
   p.g2 = dv;
   if (!host::launch_early(bwd::attn_bwd_kernel<false>, static_cast<unsigned>(kv_items < sms ? kv_items : sms),

@@ -21,7 +21,7 @@
 // needs.  In exchange dQ is not accumulated across CTAs: no atomics (the result does not
 // depend on the order in which CTAs run), no fp32 dQ in memory, and neither P nor dS ever
 // leaves TMEM.  Per tile the tensor pipe needs 2048 (dK/dV) and 1536 (dQ) cycles, and the
-// 256 softmax threads' work on it overlaps, phase against phase:
+// 512 softmax threads' work on it overlaps, phase against phase:
 //
 //   dK/dV:  tensor   | dV_n  S_{n+1} | dK_n  dP_{n+1} | dV_{n+1} ...
 //           softmax  | dS_n from dP_n | P_{n+1} from S_{n+1} | ...
@@ -37,9 +37,9 @@
 // Sums are fp32 in TMEM; P and dS are rounded once to bf16 (the type of the tensor cores'
 // operands: half a step, 2^-9 of each value), the gradients once at the end.
 //
-// Roles (512 threads): warps 0-7 softmax (two warpgroups, 64 of a tile's 128 columns each),
-// warps 8-11 the epilogue (an item's accumulators to memory, and Q of the next item to TMEM,
-// while the tile loop runs), warp 12 TMA producer, warp 13 MMA issuer, warp 14 waiter: the
+// Roles (768 threads): warps 0-15 softmax (four warpgroups, 32 of a tile's 128 columns each),
+// warps 16-19 the epilogue (an item's accumulators to memory, and Q of the next item to TMEM,
+// while the tile loop runs), warp 20 TMA producer, warp 21 MMA issuer, warp 22 waiter: the
 // issuer waits on hardware named barriers only, because a shared-memory read by the issuing
 // thread drains its queued MMAs first.  Every wait is bounded by the watchdog, and after an
 // abort every role still takes its fixed number of barrier rounds, so no CTA is left waiting.
@@ -47,25 +47,27 @@
 
 #include <cuda_bf16.h>
 
+#include <climits>
+
 #include "attn_fwd.cuh"
 
 namespace avo_b200 {
 namespace bwd {
 
 constexpr int kTile = 128;
-constexpr int kSoftmaxThreads = 256;
-constexpr int kEpiWarp = 8;
-constexpr int kProducerWarp = 12;
-constexpr int kIssuerWarp = 13;
-constexpr int kWaiterWarp = 14;
-constexpr int kBwdThreads = 512;
-// Launched at 128 registers per thread (512 x 128 = 65536); 256 x 168 + 128 x 96 + 128 x 72
-// = 64512 after the split.
-constexpr uint32_t kBwdRegsLaunch = 128;
-constexpr uint32_t kBwdRegsSoftmax = 168;
-constexpr uint32_t kBwdRegsEpi = 96;
-constexpr uint32_t kBwdRegsOther = 72;
-static_assert(256 * kBwdRegsSoftmax + 128 * kBwdRegsEpi + 128 * kBwdRegsOther <= kBwdThreads * kBwdRegsLaunch,
+constexpr int kSoftmaxThreads = 512;
+constexpr int kEpiWarp = 16;
+constexpr int kProducerWarp = 20;
+constexpr int kIssuerWarp = 21;
+constexpr int kWaiterWarp = 22;
+constexpr int kBwdThreads = 768;
+// Launched at 80 registers per thread (768 x 80 = 61440); after the split 512 x 88 + 128 x 80
+// + 128 x 48 = 61440.
+constexpr uint32_t kBwdRegsLaunch = 80;
+constexpr uint32_t kBwdRegsSoftmax = 88;
+constexpr uint32_t kBwdRegsEpi = 80;
+constexpr uint32_t kBwdRegsOther = 48;
+static_assert(kSoftmaxThreads * kBwdRegsSoftmax + 128 * kBwdRegsEpi + 128 * kBwdRegsOther <= kBwdThreads * kBwdRegsLaunch,
               "register split");
 
 // A wait that lasts as long as an item of `tiles` tiles: one lane polls, asleep in between,
@@ -92,7 +94,7 @@ __device__ __forceinline__ bool wait_item(uint32_t bar, uint32_t parity, int til
 // item): an arrival is then never counted to a round that the issuer has not reached, also
 // after an abort, when a warp no longer waits for the MMAs that order the rounds.
 //   3             first tile's operands loaded (waiter)
-//   dK/dV: 4/7, 5/8  halves of P in TMEM (8 softmax warps; 5/8: and the waiter, next T1's operand)
+//   dK/dV: 4/7, 5/8  halves of P in TMEM (softmax warps; 5/8: and the waiter, next T1's operand)
 //          6/9       dS in TMEM (softmax, and the waiter: next T2's operand)
 //          10/11, 12/13  accumulator 1 / 2 read out (epilogue warps)
 //   dQ:    4/7, 5/8  T1 / T2 in registers (softmax, and the waiter: next T1's / T2's operand)
@@ -128,7 +130,8 @@ constexpr int kStatBytes = 2 * kTile * 4;
 constexpr int kSmBars = kSmStat + 2 * kStatBytes;
 // mbarriers.  The issuer commits after T1 and after T2 of a tile, and these commits also tell
 // the producer that the MMAs issued before them are done with their operands (a commit takes
-// about 50 cycles of the issuer's time).  Only dQ's Y1 slots have a commit of their own.
+// about 50 cycles of the issuer's time).  dQ's Y1 slots and dK/dV's Y2 slots have a commit of
+// their own: with T1's, 512 cycles later, the next load into the slot came too late.
 // T1_FULL and T2_FULL are pairs, used by even and odd tiles, so that no wait can miss a phase.
 enum : int {
   B_X1_FULL = 0,
@@ -137,7 +140,8 @@ enum : int {
   B_Y1_FULL,
   B_Y1_EMPTY = B_Y1_FULL + 4,
   B_Y2_FULL = B_Y1_EMPTY + 4,
-  B_T1_FULL = B_Y2_FULL + kY2,
+  B_Y2_EMPTY = B_Y2_FULL + kY2,
+  B_T1_FULL = B_Y2_EMPTY + kY2,
   B_T2_FULL = B_T1_FULL + 2,
   B_ACC1 = B_T2_FULL + 2,
   B_ACC2,
@@ -168,6 +172,7 @@ struct BwdParams {
   int causal;
   int offset;              // causal: key j is visible to query i iff j <= i + offset
   float scale, scale_log2;
+  int overlap;             // the two passes may run at the same time
   int test_skip_load;
 };
 
@@ -270,7 +275,7 @@ __device__ __forceinline__ void issue_xy_tmem(uint32_t d_tmem, uint32_t x_tmem, 
 }
 
 // acc (+)= A Y over 64 of the 128 streamed rows: A (P or dS, bf16) from TMEM, Y from shared
-// memory as an MN-major operand.  Each softmax warpgroup holds 32 columns of either half; in
+// memory as an MN-major operand.  Each softmax warpgroup holds 16 columns of either half; in
 // dK/dV its values replace the scores at the place they came from, in dQ they lie packed.
 template <bool kPacked>
 __device__ __forceinline__ void issue_acc_half(uint32_t d_tmem, uint32_t a_tmem, uint32_t y_lo, int half,
@@ -279,7 +284,7 @@ __device__ __forceinline__ void issue_acc_half(uint32_t d_tmem, uint32_t a_tmem,
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int kk = half * 4 + q;
-    mma_ts_lo(d_tmem, a_tmem + (kPacked ? kk * 8 : (kk >> 1) * 32 + (kk & 1) * 8), y_lo + ((kk * 16 * 128) >> 4),
+    mma_ts_lo(d_tmem, a_tmem + (kPacked ? kk * 8 : kk * 16), y_lo + ((kk * 16 * 128) >> 4),
               kDescHiSw128, idesc, accumulate | (kk > 0 ? 1u : 0u));
   }
 }
@@ -290,13 +295,15 @@ __device__ __forceinline__ void issue_acc(uint32_t d_tmem, uint32_t a_tmem, uint
   issue_acc_half<kPacked>(d_tmem, a_tmem, y_lo, 1, accumulate);
 }
 
-// 2^x for pair number `i` of a chunk: kEmu of every 8 pairs on the FMA pipe (results below
-// 2^-125 become 0), the others on the MUFU unit.
-template <int kEmu>
+constexpr int kEmu = 2;
+
+// 2^x for pair number `i` of a chunk: kOf8 of every 8 pairs on the FMA pipe (results below
+// 2^-125 become 0: a hidden key's P is exactly 0 on both paths), the others on the MUFU unit.
+template <int kOf8>
 __device__ __forceinline__ uint64_t exp2_pair(int i, uint64_t x2) {
   float x0, x1, p0, p1;
   f2_unpack(x2, x0, x1);
-  if ((i & 7) < kEmu) {
+  if ((i & 7) < kOf8) {
     exp2_poly_x2(x2, p0, p1);
     p0 = x0 < -125.f ? 0.f : p0;
     p1 = x1 < -125.f ? 0.f : p1;
@@ -311,12 +318,6 @@ __device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
   float a, b;
   f2_unpack(v, a, b);
   return pack_bf16x2(a, b);
-}
-
-// 16 packed words to 16 TMEM columns.
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&w)[16]) {
-  tmem_st8(taddr, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
-  tmem_st8(taddr + 8, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
 }
 
 template <bool kDq>
@@ -361,24 +362,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // The dK/dV launch follows stats_kernel and waits for it here.  The dQ launch follows the
   // dK/dV launch, reads nothing that it writes, and can only start once all CTAs of that
-  // launch have passed this wait: it runs on the multiprocessors that launch leaves free
-  // and waits for it at its own end.
-  if (!kDq) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-  }
+  // launch have passed this wait.  With p.overlap it runs at the same time, on the
+  // multiprocessors that launch leaves free, and waits for it at its own end.
+  if (!kDq || !p.overlap) grid_dependency_wait();
+  if (!kDq) grid_launch_dependents();
 
   if (warp < kEpiWarp) {
     regs_increase<kBwdRegsSoftmax>();
     // ------------------------------------------------------------ softmax
-    // Each warpgroup takes 32 columns of either half of the tile: [32 wg, 32 wg + 32) and
+    // Each warpgroup takes 16 columns of either half of the tile: [16 wg, 16 wg + 16) and
     // 64 further on.
     const int wg = warp >> 2;
     const int wq = warp & 3;
     const int row = threadIdx.x & 127;
-    const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 32;
+    const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 16;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-    bool ok = true;
     uint32_t n = 0;
     float neg_lse = 0.f, neg_delta = 0.f;
     Tiles<kDq> it(p);
@@ -405,57 +403,60 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       next_delta = __ldg(st + kTile + row);
     };
     if (kDq) load_stats();
-    for (; it.next(); ++n) {
-      if (!ok) {
-        keep_rounds(0);
-        continue;
-      }
-      const uint32_t tT1 = tBase + kColT1, tT2 = tBase + kColT2;
-      // Columns [lo, hi) of this tile are visible to this row; mask_tile: some row of the
-      // warp does not see all of this warpgroup's columns.
-      int lo = 0, hi = kTile;
-      bool mask_tile;
-      if (kDq) {
-        const int q = it.items.tile * kTile + row;
-        const int key0 = it.t * kTile;
-        hi = p.seq_kv - key0;
-        int hi_warp = hi;
-        if (p.causal) {
-          hi = min(hi, q + p.offset - key0 + 1);
-          hi_warp = min(hi_warp, q - lane + p.offset - key0 + 1);
-        }
-        mask_tile = hi_warp < kTile;
-        if (it.first) {
-          neg_lse = next_lse;
-          neg_delta = next_delta;
-          load_stats();
-        }
-      } else {
-        const int key = it.items.tile * kTile + row;
-        lo = p.causal ? key - p.offset - it.t * kTile : 0;
-        mask_tile = p.causal && key - lane + 31 - p.offset - it.t * kTile > 0;
-      }
+    const uint32_t tT1 = tBase + kColT1, tT2 = tBase + kColT2;
+    int full_lo = 0, full_hi = 0;
+    // One tile.  Returns -1, or the first of the tile's barrier rounds that an abort kept it
+    // from.
+    auto one_tile = [&](bool masked) -> int {
       const uint32_t phase = (n >> 1) & 1;
-      ok = wait_phase(bar(B_T1_FULL + static_cast<int>(n & 1)), phase, watch);
-      if (!kDq) ok = ok && wait_phase(bar(B_STAT + static_cast<int>(n & 1)), phase, watch);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        keep_rounds(0);
-        continue;
+      bool ok;
+      {
+        const uint32_t t1 = bar(B_T1_FULL + static_cast<int>(n & 1)), st = bar(B_STAT + static_cast<int>(n & 1));
+        if (kDq) {
+          ok = wait_phase(t1, phase, watch);
+        } else {
+          // Both probes in flight together: usually both have completed.
+          const uint32_t a = mbar_try_wait(t1, phase), b = mbar_try_wait(st, phase);
+          ok = (a && b) || (wait_phase(t1, phase, watch) && wait_phase(st, phase, watch));
+        }
       }
+      if (!__all_sync(0xffffffffu, ok)) return 0;
       tc_fence_after();
       AVO_TRACE_HOOK(wg, n, 0);
+      // A tile that some row of the warp does not see whole: hidden scores become -inf in
+      // place, so that the code below is the same for every tile.  (Measured on B200, B4 H16
+      // S4096, both passes: a test behind the exponentials or a second copy of the code cost
+      // 7 to 20 %: the one splits the block that the scheduler interleaves, the other spills.)
+      if (masked) {
+        const int r = it.items.tile * kTile + row, c0 = it.t * kTile;
+        const int lo = kDq ? 0 : r - p.offset - c0;
+        const int hi = kDq ? (p.causal ? min(p.seq_kv, r + p.offset + 1) : p.seq_kv) - c0 : kTile;
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 64) {
+          uint32_t s[16];
+          tmem_ld16(tT1 + c, s);
+          tmem_wait_ld16(s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int col = c + wg * 16 + i;
+            s[i] = col >= lo && col < hi ? s[i] : 0xff800000u;
+          }
+          tmem_st8(tT1 + c, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
+          tmem_st8(tT1 + c + 8, s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15]);
+        }
+        tc_wait_st();
+      }
       // P: fp32 pairs kept for dS, bf16 to TMEM (dK/dV only) a half at a time, so that dV's
       // first MMAs overlap the second half's exponentials.
-      uint64_t pr[32];
+      uint64_t pr[16];
       {
-        uint32_t s[2][32];
-        tmem_ld32(tT1, s[0]);
-        tmem_ld32(tT1 + 64, s[1]);
-        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + wg * 128;
+        uint32_t s[2][16];
+        tmem_ld16(tT1, s[0]);
+        tmem_ld16(tT1 + 64, s[1]);
+        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + wg * 64;
         const uint64_t neg2 = f2_pack(neg_lse, neg_lse);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
+        tmem_wait_ld16(s[0]);
+        tmem_wait_ld16(s[1]);
         if (kDq) {
           // S_{n+1} may overwrite T1.
           tc_fence_before();
@@ -466,30 +467,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
+          for (int e = 0; e < 8; e += 2) {
             uint64_t la = neg2, lb = neg2;
             if (!kDq) lds_f2x2(stat + (c * 64 + e * 2) * 4, la, lb);
-            pr[c * 16 + e] =
-                exp2_pair<2>(e, f2_fma(f2_pack(u2f(s[c][2 * e]), u2f(s[c][2 * e + 1])), scale2, la));
-            pr[c * 16 + e + 1] =
-                exp2_pair<2>(e + 1, f2_fma(f2_pack(u2f(s[c][2 * e + 2]), u2f(s[c][2 * e + 3])), scale2, lb));
-          }
-          if (mask_tile) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float a, b;
-              f2_unpack(pr[c * 16 + i], a, b);
-              const int col = c * 64 + wg * 32 + 2 * i;
-              a = (col >= lo && col < hi) ? a : 0.f;
-              b = (col + 1 >= lo && col + 1 < hi) ? b : 0.f;
-              pr[c * 16 + i] = f2_pack(a, b);
-            }
+            pr[c * 8 + e] = exp2_pair<kEmu>(e, f2_fma(f2_pack(u2f(s[c][2 * e]), u2f(s[c][2 * e + 1])), scale2, la));
+            pr[c * 8 + e + 1] =
+                exp2_pair<kEmu>(e + 1, f2_fma(f2_pack(u2f(s[c][2 * e + 2]), u2f(s[c][2 * e + 3])), scale2, lb));
           }
           if (!kDq) {
-            uint32_t w[16];
+            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack_pair(pr[c * 16 + i]);
-            tmem_st16(tT1 + c * 64, w);
+            for (int i = 0; i < 8; ++i) w[i] = pack_pair(pr[c * 8 + i]);
+            tmem_st8(tT1 + c * 64, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -498,50 +487,44 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       AVO_TRACE_HOOK(wg, n, 2);
-      ok = __all_sync(0xffffffffu, wait_phase(bar(B_T2_FULL + static_cast<int>(n & 1)), phase, watch));
-      if (!ok) {
-        keep_rounds(1);
-        continue;
-      }
+      if (!__all_sync(0xffffffffu, wait_phase(bar(B_T2_FULL + static_cast<int>(n & 1)), phase, watch))) return 1;
       tc_fence_after();
       AVO_TRACE_HOOK(wg, n, 3);
       {
-        uint32_t d[2][32];
-        tmem_ld32(tT2, d[0]);
-        tmem_ld32(tT2 + 64, d[1]);
-        tmem_wait_ld(d[0]);
-        tmem_wait_ld(d[1]);
+        uint32_t d[2][16];
+        tmem_ld16(tT2, d[0]);
+        tmem_ld16(tT2 + 64, d[1]);
+        tmem_wait_ld16(d[0]);
+        tmem_wait_ld16(d[1]);
         if (kDq) {
           // dP_{n+1} may overwrite T2 while dS_n is computed.
           tc_fence_before();
           __syncwarp();
           named_bar_arrive(bar_tile(kRoundT2Read, n), kTileThreads);
         }
-        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + kTile * 4 + wg * 128;
+        const uint32_t stat = sbase + kSmStat + (n & 1) * kStatBytes + kTile * 4 + wg * 64;
         const uint64_t neg2 = f2_pack(neg_delta, neg_delta);
-        const uint32_t tDs = kDq ? tBase - wg * 16 + kColDs : tT2;
+        const uint32_t tDs = kDq ? tBase - wg * 8 + kColDs : tT2;
         if (kDq && n > 0) {
           // dQ_{n-1} has read the previous dS.
           const uint32_t u = n - 1;
-          ok = __all_sync(0xffffffffu, wait_phase(bar(B_Y1_EMPTY + static_cast<int>(u % kY1)), (u / kY1) & 1, watch));
-          if (!ok) {
-            keep_rounds(2);
-            continue;
-          }
+          if (!__all_sync(0xffffffffu,
+                          wait_phase(bar(B_Y1_EMPTY + static_cast<int>(u % kY1)), (u / kY1) & 1, watch)))
+            return 2;
           tc_fence_after();
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t w[16];
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
+          for (int e = 0; e < 8; e += 2) {
             uint64_t la = neg2, lb = neg2;
             if (!kDq) lds_f2x2(stat + (c * 64 + e * 2) * 4, la, lb);
-            w[e] = pack_pair(f2_mul(pr[c * 16 + e], f2_add(f2_pack(u2f(d[c][2 * e]), u2f(d[c][2 * e + 1])), la)));
+            w[e] = pack_pair(f2_mul(pr[c * 8 + e], f2_add(f2_pack(u2f(d[c][2 * e]), u2f(d[c][2 * e + 1])), la)));
             w[e + 1] = pack_pair(
-                f2_mul(pr[c * 16 + e + 1], f2_add(f2_pack(u2f(d[c][2 * e + 2]), u2f(d[c][2 * e + 3])), lb)));
+                f2_mul(pr[c * 8 + e + 1], f2_add(f2_pack(u2f(d[c][2 * e + 2]), u2f(d[c][2 * e + 3])), lb)));
           }
-          tmem_st16(tDs + c * (kDq ? 32 : 64), w);
+          tmem_st8(tDs + c * (kDq ? 32 : 64), w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
         }
       }
       tc_wait_st();
@@ -549,43 +532,72 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       named_bar_arrive(bar_tile(kRoundDs, n), kDsThreads<kDq>);
       AVO_TRACE_HOOK(wg, n, 4);
+      return -1;
+    };
+    int failed = -1;
+    for (; it.next(); ++n) {
+      if (it.first) {
+        // Every row of the warp sees all columns of the tiles from full_lo up to full_hi.
+        const int r0 = it.items.tile * kTile + wq * 32;  // the warp's first row
+        full_lo = 0;
+        full_hi = INT_MAX;
+        if (kDq) {
+          full_hi = p.causal ? max(0, min(p.seq_kv, r0 + p.offset + 1)) / kTile : p.seq_kv / kTile;
+          neg_lse = next_lse;
+          neg_delta = next_delta;
+          load_stats();
+        } else if (p.causal) {
+          full_lo = (max(0, r0 + 31 - p.offset) + kTile - 1) / kTile;
+        }
+      }
+      failed = one_tile(it.t < full_lo || it.t >= full_hi);
+      if (failed >= 0) break;
+    }
+    if (failed >= 0) {
+      keep_rounds(failed);
+      for (++n; it.next(); ++n) keep_rounds(0);
     }
   } else if (warp < kProducerWarp) {
-    regs_decrease<kBwdRegsEpi>();
+    if constexpr (kBwdRegsEpi < kBwdRegsLaunch) regs_decrease<kBwdRegsEpi>();
     // ------------------------------------------------------------ epilogue
     const int row = threadIdx.x & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int rows = kDq ? p.seq_q : p.seq_kv;
     bool ok = true;
     uint32_t done = 0;   // items with tiles so far
-    // dQ: this thread's row of Q of the next item with tiles, loaded an item ahead.
+    // dQ: this thread's row of Q of the next item with tiles, its first half loaded an item
+    // ahead, the second when it is stored.
     Items<kDq> ahead(p);
-    uint32_t xq[64];
+    uint32_t xq[32];
     bool have_x = false;
+    auto load_half = [&](int half) {
+      const int r = ahead.tile * kTile + row;
+      const bool valid = r < rows;
+      const uint4* src =
+          static_cast<const uint4*>(p.x1) + (static_cast<long long>(ahead.head) * rows + (valid ? r : 0)) * 16 + half * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 v = valid ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+        xq[4 * i] = v.x;
+        xq[4 * i + 1] = v.y;
+        xq[4 * i + 2] = v.z;
+        xq[4 * i + 3] = v.w;
+      }
+    };
     auto load_x = [&]() {
       have_x = ahead.next_busy();
-      const int r = ahead.tile * kTile + row;
-      if (have_x && r < rows) {
-        const uint4* src = static_cast<const uint4*>(p.x1) + (static_cast<long long>(ahead.head) * rows + r) * 16;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint4 v = __ldg(src + i);
-          xq[4 * i] = v.x;
-          xq[4 * i + 1] = v.y;
-          xq[4 * i + 2] = v.z;
-          xq[4 * i + 3] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) xq[i] = 0u;
-      }
+      if (have_x) load_half(0);
     };
     uint32_t x_signals = 0, acc_signals = 0;
     auto store_x = [&]() {
-      const uint32_t t = tmem + lane_off + kColX1;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        if (half == 1) load_half(1);
+        const uint32_t t = tmem + lane_off + kColX1 + half * 32;
 #pragma unroll
-      for (int i = 0; i < 64; i += 8)
-        tmem_st8(t + i, xq[i], xq[i + 1], xq[i + 2], xq[i + 3], xq[i + 4], xq[i + 5], xq[i + 6], xq[i + 7]);
+        for (int i = 0; i < 32; i += 8)
+          tmem_st8(t + i, xq[i], xq[i + 1], xq[i + 2], xq[i + 3], xq[i + 4], xq[i + 5], xq[i + 6], xq[i + 7]);
+      }
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -622,16 +634,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tc_fence_after();
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[16];
           if (it.n > 0) {
-            tmem_ld32(acc + c * 32, o);
-            tmem_wait_ld(o);
+            tmem_ld16(acc + c * 16, o);
+            tmem_wait_ld16(o);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 16; ++e) o[e] = 0u;
           }
-          if (c == 3 && it.n > 0) {
+          if (c == 7 && it.n > 0) {
             // Read out: the next item may overwrite it.
             tc_fence_before();
             __syncwarp();
@@ -639,14 +651,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             ++acc_signals;
           }
           if (write) {
+            uint32_t w[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t w[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                w[e] = pack_bf16x2(u2f(o[16 * q + 2 * e]) * f, u2f(o[16 * q + 2 * e + 1]) * f);
-              st_global_v8(dst + c * 32 + q * 16, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
-            }
+            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(u2f(o[2 * e]) * f, u2f(o[2 * e + 1]) * f);
+            st_global_v8(dst + c * 16, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
           }
         }
       }
@@ -733,9 +741,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           load(Sm::kX1, &tm_x1, B_X1_FULL, it.items.tile * kTile, it.items.head, pol_x);
           ++nx1;
         }
-        // Y2's last user is dV, before T1 of the next tile (dK/dV), or T2 itself (dQ).
-        if (n2 >= kY2 && !reuse(kDq ? B_T2_FULL : B_T1_FULL, kDq ? last - 1 : last, B_Y2_FULL + s2, (n2 / kY2 - 1) & 1))
-          break;
+        // Y2's last user is dV, or T2 itself (dQ).
+        if (n2 >= kY2) {
+          const uint32_t before = (n2 / kY2 - 1) & 1;
+          if (!(kDq ? reuse(B_T2_FULL, last - 1, B_Y2_FULL + s2, before)
+                    : reuse_after(B_Y2_EMPTY + s2, before, B_Y2_FULL + s2, before)))
+            break;
+        }
         load(Sm::kY2At + s2 * kTileBytes, &tm_y2, B_Y2_FULL + s2, it.t * kTile, it.y_head, pol_y);
         ++n2;
         if (it.first) {
@@ -820,6 +832,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         sync_on(bar_tile(kRoundP1, par), kTileThreads);
         if (leader) {
           issue_acc_half<false>(tA2, tT1, y2t + par * kSlot, 1, 1u);
+          mma_commit(bar(B_Y2_EMPTY + par));
           if (last) mma_commit(bar(B_ACC2));
           if (have) issue_t1(n1, other);
         }
@@ -904,7 +917,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       round(bar_tile(kDq ? kRoundT2Read : kRoundDs, n), kTileThreads);
     }
   } else {
-    regs_decrease<kBwdRegsOther>();  // warp 15 completes the warpgroup
+    regs_decrease<kBwdRegsOther>();  // warp 23 completes the warpgroup
   }
 
   tc_fence_before();
@@ -914,7 +927,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_dealloc(tmem, kTmemCols);
   }
   // The dQ launch is complete only when the dK/dV launch is (see above).
-  if (kDq) grid_dependency_wait();
+  if (kDq && p.overlap) grid_dependency_wait();
 }
 
 // -LSE*log2(e) and -delta of every query row, padded to whole tiles: [heads][nq][2][128].

@@ -105,7 +105,7 @@ class BwdModel(Model):
                 self.load("X1", "X1_FULL", item)
             if n >= Y2:
                 if self.fault != "no_y2_wait":
-                    yield self.t_full(2, n - 2) if self.dq else self.t_full(1, n - 1)
+                    yield self.t_full(2, n - 2) if self.dq else self.wait(f"Y2_EMPTY{s2}", n // Y2 - 1)
                 yield self.wait(f"Y2_FULL{s2}", n // Y2 - 1)
             if self.aborted:
                 return
@@ -200,6 +200,8 @@ class BwdModel(Model):
         self.op(run)
         if self.dq and half == 1:
             self.commit(f"Y1_EMPTY{n % self.y1}")
+        if which == 2 and half == 1:
+            self.commit(f"Y2_EMPTY{n % Y2}")
         if last and half == 1:
             self.commit(f"ACC{which}")
 
