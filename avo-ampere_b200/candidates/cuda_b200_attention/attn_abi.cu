@@ -469,16 +469,43 @@ extern "C" int avo_b200_attn_fwd(const void* q, const void* k, const void* v, vo
 
 extern "C" int avo_b200_attn_fwd_grouped(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
                                          int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
-                                         float softmax_scale, int* status_dev, void* stream) {
+                                         float softmax_scale, void* workspace, size_t workspace_bytes,
+                                         int* status_dev, void* stream) {
   if (batch < 0 || heads < 0 || kv_heads <= 0 || seq_q < 0 || seq_kv < 0 || heads % kv_heads != 0)
     return AVO_B200_EINVAL;
   const long long bh = static_cast<long long>(batch) * heads;
   if (bh > INT_MAX) return AVO_B200_EINVAL;
+  int group = heads / kv_heads;
+  long long pairs = bh;
+  if (seq_q == 1 && seq_kv > 0) causal = 0;  // a single query sees every key
+  if (!causal && group > 1 && static_cast<long long>(group) * seq_q <= INT_MAX / 2) {
+    // Without a mask the rows of the heads that share a key/value head attend alike, and they
+    // are adjacent in memory: one head of group * seq_q rows, whose keys are read once.
+    seq_q *= group;
+    pairs = static_cast<long long>(batch) * kv_heads;
+    group = 1;
+  }
   const long long qhs = static_cast<long long>(seq_q) * kHeadDim, khs = static_cast<long long>(seq_kv) * kHeadDim;
-  // Query row i sits at position seq_kv - seq_q + i: the last query sees every key.
-  return launch_fwd(q, k, v, o, lse, static_cast<int>(bh), seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim, qhs,
-                    seq_q, causal, softmax_scale, static_cast<long long>(seq_kv) - seq_q, 0, status_dev, stream,
-                    nullptr, 0, heads > 0 ? heads / kv_heads : 1);
+  if (workspace != nullptr && bh > 0 && seq_q > 0 && head_dim == kHeadDim) {
+    // Only the split plan uses the workspace; its flags (at the front) have to start at zero.
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return AVO_B200_EINVAL;
+    int sms = 0;
+    const int rc = prepare_device(&sms);
+    if (rc != AVO_B200_OK) return rc;
+    if (workspace_bytes < workspace_bytes_for(sms)) return AVO_B200_EINVAL;
+    const long long items = pairs * ((static_cast<long long>(seq_q) + kRowsPerCta - 1) / kRowsPerCta);
+    if (items <= INT_MAX && !causal && cooperative_ok() &&
+        cached_plan(static_cast<int>(pairs), seq_q, seq_kv, 0, 0, 0, sms, true).plan.mode == sched::kTail &&
+        cudaMemsetAsync(workspace, 0, static_cast<size_t>(sms) * kFlagBytesPerCta, static_cast<cudaStream_t>(stream)) !=
+            cudaSuccess) {
+      (void)cudaGetLastError();
+      return AVO_B200_ELAUNCH;
+    }
+  }
+  // With a mask, query row i sits at position seq_kv - seq_q + i: the last query sees every key.
+  return launch_fwd(q, k, v, o, lse, static_cast<int>(pairs), seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim,
+                    qhs, seq_q, causal, softmax_scale, causal ? static_cast<long long>(seq_kv) - seq_q : 0, 0,
+                    status_dev, stream, workspace, workspace_bytes, group);
 }
 
 extern "C" int avo_b200_attn_workspace_size(size_t* bytes) {

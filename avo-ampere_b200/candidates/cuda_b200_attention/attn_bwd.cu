@@ -52,6 +52,17 @@ bool sizes_ok(int batch, int heads, int kv_heads, int seq_q, int seq_kv) {
   return qh * nq <= INT_MAX && qh * nkv <= INT_MAX && (heads / kv_heads) * nq <= INT_MAX;
 }
 
+// Without a mask, and for a single query, the rows of the query heads that share a key/value
+// head attend alike, and they are adjacent in memory: one head of group * seq_q rows.  Fewer
+// partly filled tiles (and none of the group's heads reads the keys again).
+void fold_group(int& heads, int kv_heads, int& seq_q, int seq_kv, int& causal) {
+  if (seq_q == 1 && seq_kv > 0) causal = 0;  // the last query sees every key
+  const long long rows = static_cast<long long>(heads / kv_heads) * seq_q;
+  if (causal || rows > INT_MAX - 2 * kTile) return;
+  seq_q = static_cast<int>(rows);
+  heads = kv_heads;
+}
+
 size_t stats_bytes(int batch, int heads, int seq_q) {
   return static_cast<size_t>(batch) * heads * tiles_of(seq_q) * bwd::kStatBytes;
 }
@@ -72,7 +83,7 @@ using namespace avo_b200;
 extern "C" int avo_b200_attn_bwd_workspace_size(int batch, int heads, int kv_heads, int seq_q, int seq_kv,
                                                 size_t* bytes) {
   if (bytes == nullptr || !sizes_ok(batch, heads, kv_heads, seq_q, seq_kv)) return AVO_B200_EINVAL;
-  *bytes = stats_bytes(batch, heads, seq_q);
+  *bytes = stats_bytes(batch, heads, seq_q);  // not less than with the group folded
   return AVO_B200_OK;
 }
 
@@ -83,6 +94,8 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   if (head_dim != kHeadDim || !sizes_ok(batch, heads, kv_heads, seq_q, seq_kv)) return AVO_B200_EINVAL;
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return AVO_B200_EINVAL;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t wanted = stats_bytes(batch, heads, seq_q);
+  fold_group(heads, kv_heads, seq_q, seq_kv, causal);
   const int q_heads = batch * heads, kv_all = batch * kv_heads;
   const size_t q_bytes = static_cast<size_t>(q_heads) * seq_q * kHeadDim * 2;
   const size_t kv_bytes = static_cast<size_t>(kv_all) * seq_kv * kHeadDim * 2;
@@ -100,7 +113,7 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   for (void* p : grads)
     if (p == nullptr || !host::aligned(p, 32)) return AVO_B200_EINVAL;
   if (lse == nullptr || !host::aligned(lse, 4)) return AVO_B200_EINVAL;
-  if (workspace == nullptr || !host::aligned(workspace, 256) || workspace_bytes < stats_bytes(batch, heads, seq_q))
+  if (workspace == nullptr || !host::aligned(workspace, 256) || workspace_bytes < wanted)
     return AVO_B200_EINVAL;
 
   int sms = 0;
@@ -124,7 +137,7 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   p.kv_heads = kv_all;
   p.group = heads / kv_heads;
   p.causal = causal ? 1 : 0;
-  p.offset = seq_kv - seq_q;
+  p.offset = causal ? seq_kv - seq_q : 0;
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.test_skip_load = host::skip_load();

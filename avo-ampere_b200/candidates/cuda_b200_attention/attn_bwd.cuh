@@ -694,15 +694,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tma_load_3d(sbase + off, tm, bar(b), 0, r0, head, pol);
         tma_load_3d(sbase + off + kHalfBytes, tm, bar(b), 64, r0, head, pol);
       };
-      // A buffer may be loaded again once its last user is done and its previous copy has
-      // landed (implied unless the CTA aborted): at most one copy per buffer is in flight.
-      auto reuse_after = [&](int done, uint32_t done_parity, int full, uint32_t full_parity) {
-        return wait_phase(bar(done), done_parity, watch) && wait_phase(bar(full), full_parity, watch) && !*abort_flag;
+      // A buffer may be loaded again once its last user is done.  That it is done also means
+      // that its previous copy has landed, unless the CTA aborted before: then the MMAs no
+      // longer waited for data.  The flag is set before any such MMA is issued, so it is seen
+      // here after its commit: at most one copy per buffer is ever in flight.  (No more than
+      // these two reads of shared memory per load: each takes 100 to 300 cycles while the MMAs
+      // read their operands.)
+      auto reuse_after = [&](int done, uint32_t parity) {
+        return wait_phase(bar(done), parity, watch) && !*abort_flag;
       };
       // ... done as tile u's T1 or T2 commit implies.
-      auto reuse = [&](int commit, int u, int full, uint32_t full_parity) {
-        return reuse_after(commit + (u & 1), (u >> 1) & 1, full, full_parity);
-      };
+      auto reuse = [&](int commit, int u) { return reuse_after(commit + (u & 1), (u >> 1) & 1); };
       int n = 0, n2 = 0, nx1 = 0, nx2 = 0, nst = 0, skipped = -1;
       // The stationary tiles of the next item, and its first streamed ones, are brought to L2
       // while this item runs: their loads start only when its last tiles are done with the
@@ -724,34 +726,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         const int s1 = n % kY1, s2 = n % kY2;
         // Y1's last user is its tile's last MMA: dQ, or dK, which precedes the next tile's T2.
-        if (n >= kY1) {
-          const uint32_t before = (n / kY1 - 1) & 1;
-          if (!(kDq ? reuse_after(B_Y1_EMPTY + s1, before, B_Y1_FULL + s1, before)
-                    : reuse(B_T2_FULL, n - 2, B_Y1_FULL + s1, before)))
-            break;
-        }
-        if (*abort_flag) break;
+        if (n >= kY1 && !(kDq ? reuse_after(B_Y1_EMPTY + s1, (n / kY1 - 1) & 1) : reuse(B_T2_FULL, n - 2))) break;
         if (n == p.test_skip_load) skipped = n;  // test hook: this copy never arrives
         if (n != skipped) load(Sm::kY1At + s1 * kTileBytes, &tm_y1, B_Y1_FULL + s1, it.t * kTile, it.y_head, pol_y);
         ++n;
         const int last = n - 2;  // the previous tile
         if (!kDq && it.first) {
           // X1 was read last by the previous tile's T1, X2 by its T2.
-          if (nx1 > 0 && !reuse(B_T1_FULL, last, B_X1_FULL, (nx1 - 1) & 1)) break;
+          if (nx1 > 0 && !reuse(B_T1_FULL, last)) break;
           load(Sm::kX1, &tm_x1, B_X1_FULL, it.items.tile * kTile, it.items.head, pol_x);
           ++nx1;
         }
         // Y2's last user is dV, or T2 itself (dQ).
-        if (n2 >= kY2) {
-          const uint32_t before = (n2 / kY2 - 1) & 1;
-          if (!(kDq ? reuse(B_T2_FULL, last - 1, B_Y2_FULL + s2, before)
-                    : reuse_after(B_Y2_EMPTY + s2, before, B_Y2_FULL + s2, before)))
-            break;
-        }
+        if (n2 >= kY2 && !(kDq ? reuse(B_T2_FULL, last - 1) : reuse_after(B_Y2_EMPTY + s2, (n2 / kY2 - 1) & 1))) break;
         load(Sm::kY2At + s2 * kTileBytes, &tm_y2, B_Y2_FULL + s2, it.t * kTile, it.y_head, pol_y);
         ++n2;
         if (it.first) {
-          if (nx2 > 0 && !reuse(B_T2_FULL, last, B_X2_FULL, (nx2 - 1) & 1)) break;
+          if (nx2 > 0 && !reuse(B_T2_FULL, last)) break;
           load(Sm::kX2, &tm_x2, B_X2_FULL, it.items.tile * kTile, it.items.head, pol_x);
           ++nx2;
         }
@@ -759,7 +750,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // The slot's last readers published dS of tile nst - 2 before that tile's dK, which
           // precedes T2 of tile nst - 1.
           const int slot = nst & 1;
-          if (nst >= 2 && !reuse(B_T2_FULL, nst - 1, B_STAT + slot, ((nst >> 1) - 1) & 1)) break;
+          if (nst >= 2 && !reuse(B_T2_FULL, nst - 1)) break;
           const float* src = p.stats + (static_cast<long long>(it.y_head) * p.nq + it.t) * (2 * kTile);
           mbar_arrive_expect_tx(bar(B_STAT + slot), kStatBytes);
           bulk_load(sbase + kSmStat + slot * kStatBytes, src, kStatBytes, bar(B_STAT + slot));

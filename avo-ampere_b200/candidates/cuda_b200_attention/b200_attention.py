@@ -61,7 +61,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
     "avo_b200_attn_fwd_grouped": (
         _c_int,
-        [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, _vp],
+        [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, ctypes.c_size_t,
+         _vp, _vp],
     ),
     "avo_b200_attn_bwd_workspace_size": (
         _c_int,

@@ -94,6 +94,18 @@ def _scale(softmax_scale) -> float:
     return scale
 
 
+_forward_scratch: dict[int, int] = {}
+
+
+def _forward_scratch_bytes(index: int) -> int:
+    """Scratch of the forward's split plan on device ``index`` (a function of the device alone)."""
+    if index not in _forward_scratch:
+        size = ctypes.c_size_t(0)
+        b._check(b.load_library().avo_b200_attn_workspace_size(ctypes.byref(size)), "avo_b200_attn_workspace_size")
+        _forward_scratch[index] = size.value
+    return _forward_scratch[index]
+
+
 def _forward(q, k, v, causal: bool, scale: float):
     torch = _torch()
     batch, heads, kv_heads, seq_q, seq_kv = _attention_shape(q, k, v)
@@ -106,9 +118,12 @@ def _forward(q, k, v, causal: bool, scale: float):
     lib = b.load_library()
     index = q.get_device()
     with _on(index):
+        size = _forward_scratch_bytes(index)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         code = lib.avo_b200_attn_fwd_grouped(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,
-            seq_kv, HEAD_DIM, 1 if causal else 0, scale, b.status_word(index).data_ptr(), b._raw_stream(index))
+            seq_kv, HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_word(index).data_ptr(),
+            b._raw_stream(index))
     b._check(code, "avo_b200_attn_fwd_grouped")
     return out, lse
 

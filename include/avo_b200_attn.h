@@ -180,12 +180,15 @@ int avo_b200_attn_fwd_split_noalloc(const void* q, const void* k, const void* v,
  * kv_heads (query head h reads key/value head h / (heads / kv_heads)); lse is fp32
  * [batch, heads, seq_q] and may be null.  causal != 0 aligns the two sequences at their
  * ends: query i sees keys j <= i + seq_kv - seq_q, so with seq_q > seq_kv the first
- * queries see none (o = 0, lse = -inf).  Whole work items only, no workspace: calls on
- * several streams share nothing.  No reference counterpart.
+ * queries see none (o = 0, lse = -inf).  workspace: null (whole work items only), or
+ * device memory of avo_b200_attn_workspace_size() bytes, 256-byte aligned, uninitialised,
+ * which lets the kernel cut items between CTAs as avo_b200_attn_fwd_ws does; calls that may
+ * overlap in time need a workspace each.  No reference counterpart.
  */
 int avo_b200_attn_fwd_grouped(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
                               int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
-                              float softmax_scale, int* status_dev, void* stream);
+                              float softmax_scale, void* workspace, size_t workspace_bytes,
+                              int* status_dev, void* stream);
 
 /*
  * Gradient of avo_b200_attn_fwd_grouped (and, with kv_heads == heads and seq_kv == seq_q,

@@ -39,6 +39,8 @@ CASES = [
     (2, 16, 16, 1280, 1280, False),  # more items than multiprocessors
     (2, 16, 8, 1300, 1300, True),
     (1, 6, 1, 1024, 129, False),
+    (1, 16, 2, 1, 3000, True),    # one token of a long context, eight heads to a key
+    (2, 9, 3, 5, 1111, False),
 ]
 
 
@@ -157,7 +159,7 @@ def test_equal_shapes_give_the_candidate_forwards_bits(b200, training):
     for case in [(1, 4, 4, 512, 512, False), (1, 4, 4, 500, 500, True)]:
         q, k, v, _ = make(case, seed=3)
         out, lse = training.grouped_attention(q, k, v, case[5])
-        want, want_lse = b200.attention_forward(q, k, v, case[5], split=False)
+        want, want_lse = b200.attention_forward(q, k, v, case[5])
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 

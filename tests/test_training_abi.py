@@ -45,13 +45,13 @@ def test_grouped_forward_refusals(b200):
     lib = b200.load_library()
 
     def call(q=FAKE, k=FAKE, v=FAKE, o=FAKE, lse=None, batch=1, heads=4, kv_heads=2, sq=64, skv=64, d=128, causal=0,
-             scale=0.088):
-        return lib.avo_b200_attn_fwd_grouped(q, k, v, o, lse, batch, heads, kv_heads, sq, skv, d, causal, scale, None,
-                                             None)
+             scale=0.088, ws=None, ws_bytes=0):
+        return lib.avo_b200_attn_fwd_grouped(q, k, v, o, lse, batch, heads, kv_heads, sq, skv, d, causal, scale, ws,
+                                             ws_bytes, None, None)
 
     for over in (dict(q=None), dict(k=None), dict(o=FAKE + 8), dict(heads=3), dict(kv_heads=0), dict(d=64),
                  dict(scale=-1.0), dict(batch=-1), dict(sq=-1), dict(skv=-1), dict(batch=2**30, heads=4),
-                 dict(lse=FAKE + 2)):
+                 dict(lse=FAKE + 2), dict(ws=FAKE + 8, ws_bytes=1 << 30)):
         assert call(**over) == INVALID, over
     assert call(batch=0) == 0 and call(sq=0) == 0
 
