@@ -103,6 +103,10 @@ _lib: ctypes.CDLL | None = None
 # to the address of the same function in the loaded library), or None where that binding
 # was not built: the ctypes call is then used.
 _fwd_ws_fast: Any = None
+# The same for the entries of the training side: _fast_call(index in FAST_ENTRIES, args...).
+_fast_call: Any = None
+FAST_ENTRIES = ("avo_b200_attn_fwd_grouped", "avo_b200_attn_bwd", "avo_b200_qkv_norm_rope",
+                "avo_b200_qkv_norm_rope_bwd")
 _status_words: dict[int, Any] = {}
 _workspaces: dict[int, Any] = {}
 
@@ -148,7 +152,7 @@ def load_library(*, build: bool = True) -> ctypes.CDLL:
 
 
 def _bind_fast(builder, lib: ctypes.CDLL) -> None:
-    global _fwd_ws_fast
+    global _fwd_ws_fast, _fast_call
     path = getattr(builder, "FAST_PATH", None)
     if path is None or not path.is_file():
         return
@@ -157,6 +161,9 @@ def _bind_fast(builder, lib: ctypes.CDLL) -> None:
     spec.loader.exec_module(module)
     module.bind(ctypes.cast(lib.avo_b200_attn_fwd_ws, ctypes.c_void_p).value)
     _fwd_ws_fast = module.fwd_ws
+    for index, name in enumerate(FAST_ENTRIES):
+        module.bind_entry(index, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
+    _fast_call = module.call
 
 
 def strerror(code: int) -> str:
@@ -206,6 +213,24 @@ def _launch_state(index: int) -> tuple[int, int, int]:
         state = (ws.data_ptr(), ws.numel(), status_word(index).data_ptr())
         _launch_states[index] = state
     return state
+
+
+def call_entry(index: int, *args) -> int:
+    """Entry FAST_ENTRIES[index] of the loaded library with plain integer and float arguments."""
+    if _fast_call is not None:
+        return _fast_call(index, *args)
+    return getattr(_lib, FAST_ENTRIES[index])(*args)
+
+
+_status_addresses: dict[int, int] = {}
+
+
+def status_address(index: int) -> int:
+    """Address of device ``index``'s status word (it lives as long as the process)."""
+    address = _status_addresses.get(index)
+    if address is None:
+        address = _status_addresses[index] = status_word(index).data_ptr()
+    return address
 
 
 def status_word(device) -> Any:

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import importlib.util
 import math
 import sys
@@ -48,14 +49,23 @@ def _torch():
     return torch
 
 
+_here = contextlib.nullcontext()
+
+
 def _on(index: int):
     """Makes device ``index`` current for a call, if it is not."""
-    cuda = _torch().cuda
-    return contextlib.nullcontext() if index == cuda.current_device() else cuda.device(index)
+    torch = _torch()
+    return _here if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def _plain(t, dtype, index: int) -> bool:
+    """A contiguous tensor of ``dtype`` on CUDA device ``index``."""
+    return t.is_cuda and t.dtype is dtype and t.get_device() == index and t.is_contiguous()
 
 
 def _check_tensors(named, dtype, device=None) -> None:
-    """CUDA, contiguous, of ``dtype``, and all on one device."""
+    """Raises what is wrong with the first tensor that is not CUDA, of ``dtype``, contiguous
+    and on ``device`` (or that of the first)."""
     for name, t in named:
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor")
@@ -72,19 +82,24 @@ def _check_tensors(named, dtype, device=None) -> None:
 
 def _attention_shape(q, k, v) -> tuple[int, int, int, int, int]:
     """(batch, heads, kv_heads, seq_q, seq_kv) of checked q, k, v."""
-    _check_tensors((("q", q), ("k", k), ("v", v)), _torch().bfloat16)
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    bf16 = _torch().bfloat16
+    index = q.get_device()
+    if not (_plain(q, bf16, index) and _plain(k, bf16, index) and _plain(v, bf16, index)):
+        _check_tensors((("q", q), ("k", k), ("v", v)), bf16)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.dim() != 4:
         raise RuntimeError("q, k, and v must have shape (batch, heads, seq, dim)")
-    if k.shape != v.shape:
+    if ks != v.shape:
         raise RuntimeError("k and v must have the same shape")
-    if q.shape[3] != HEAD_DIM or k.shape[3] != HEAD_DIM:
+    batch, heads, seq_q, dim = qs
+    kv_batch, kv_heads, seq_kv, kv_dim = ks
+    if dim != HEAD_DIM or kv_dim != HEAD_DIM:
         raise RuntimeError(f"head_dim must be {HEAD_DIM}")
-    if q.shape[0] != k.shape[0]:
+    if batch != kv_batch:
         raise RuntimeError("q and k must have the same batch")
-    heads, kv_heads = q.shape[1], k.shape[1]
     if kv_heads == 0 or heads % kv_heads != 0:
         raise RuntimeError("the query heads must be a multiple of the key/value heads")
-    return q.shape[0], heads, kv_heads, q.shape[2], k.shape[2]
+    return batch, heads, kv_heads, seq_q, seq_kv
 
 
 def _scale(softmax_scale) -> float:
@@ -115,14 +130,14 @@ def _forward(q, k, v, causal: bool, scale: float):
         return out, lse
     if seq_kv == 0:
         return out.zero_(), lse.fill_(-math.inf)
-    lib = b.load_library()
+    b.load_library()
     index = q.get_device()
     with _on(index):
         size = _forward_scratch_bytes(index)
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
-        code = lib.avo_b200_attn_fwd_grouped(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,
-            seq_kv, HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_word(index).data_ptr(),
+        code = b.call_entry(
+            0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,
+            seq_kv, HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_address(index),
             b._raw_stream(index))
     b._check(code, "avo_b200_attn_fwd_grouped")
     return out, lse
@@ -192,6 +207,16 @@ def grouped_attention(q, k, v, causal: bool, *, softmax_scale: float | None = No
     return _forward(q, k, v, causal, scale)
 
 
+@functools.lru_cache(maxsize=256)
+def _backward_scratch_bytes(batch: int, heads: int, kv_heads: int, seq_q: int, seq_kv: int) -> int:
+    """Scratch of the backward for these sizes."""
+    size = ctypes.c_size_t(0)
+    b._check(b.load_library().avo_b200_attn_bwd_workspace_size(batch, heads, kv_heads, seq_q, seq_kv,
+                                                               ctypes.byref(size)),
+             "avo_b200_attn_bwd_workspace_size")
+    return size.value
+
+
 def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: float | None = None, dq=None,
                        dk=None, dv=None):
     """(dq, dk, dv), bf16, of ``out = attention(q, k, v)`` for the gradient ``dout`` of out.
@@ -204,35 +229,32 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
     torch = _torch()
     batch, heads, kv_heads, seq_q, seq_kv = _attention_shape(q, k, v)
     scale = _scale(softmax_scale)
-    _check_tensors((("dout", dout), ("out", out)), torch.bfloat16, q.device)
-    _check_tensors((("lse", lse),), torch.float32, q.device)
-    for name, t in (("dout", dout), ("out", out)):
-        if t.shape != q.shape:
-            raise RuntimeError(f"{name} must have the shape of q")
-    if tuple(lse.shape) != (batch, heads, seq_q):
+    index = q.get_device()
+    if not (_plain(dout, torch.bfloat16, index) and _plain(out, torch.bfloat16, index)):
+        _check_tensors((("dout", dout), ("out", out)), torch.bfloat16, q.device)
+    if not _plain(lse, torch.float32, index):
+        _check_tensors((("lse", lse),), torch.float32, q.device)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise RuntimeError(f"{'out' if dout.shape == q.shape else 'dout'} must have the shape of q")
+    if lse.shape != q.shape[:3]:
         raise RuntimeError("lse must have shape (batch, heads, seq)")
-    grads = []
     for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t is None:
-            t = torch.empty_like(like)
-        else:
+        if t is not None:
             _check_tensors(((name, t),), torch.bfloat16, q.device)
             if t.shape != like.shape:
                 raise RuntimeError(f"{name} must have the shape of {name[1:]}")
-        grads.append(t)
-    lib = b.load_library()
-    size = ctypes.c_size_t(0)
-    b._check(lib.avo_b200_attn_bwd_workspace_size(batch, heads, kv_heads, seq_q, seq_kv, ctypes.byref(size)),
-             "avo_b200_attn_bwd_workspace_size")
-    index = q.get_device()
+    grads = (torch.empty_like(q) if dq is None else dq, torch.empty_like(k) if dk is None else dk,
+             torch.empty_like(v) if dv is None else dv)
     with _on(index):
-        scratch = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-        code = lib.avo_b200_attn_bwd(
-            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            *(t.data_ptr() for t in grads), batch, heads, kv_heads, seq_q, seq_kv, HEAD_DIM, 1 if causal else 0,
-            scale, scratch.data_ptr(), size.value, b.status_word(index).data_ptr(), b._raw_stream(index))
+        size = _backward_scratch_bytes(batch, heads, kv_heads, seq_q, seq_kv)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        code = b.call_entry(
+            1, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), batch, heads, kv_heads, seq_q, seq_kv,
+            HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_address(index),
+            b._raw_stream(index))
     b._check(code, "avo_b200_attn_bwd")
-    return tuple(grads)
+    return grads
 
 
 # ---------------------------------------------------------------- QKV norm + rotation
@@ -251,22 +273,28 @@ def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, pos
         raise RuntimeError("the numbers of heads must not be negative")
     if qkv.dim() != 4 or qkv.shape[2] != heads + 2 * kv_heads or qkv.shape[3] != HEAD_DIM:
         raise RuntimeError(f"qkv must have shape (batch, seq, heads + 2 * kv_heads, {HEAD_DIM})")
-    batch, seq = qkv.shape[0], qkv.shape[1]
-    if qkv.numel() and (qkv.stride(3) != 1 or (qkv.shape[2] > 1 and qkv.stride(2) != HEAD_DIM)):
+    batch, seq, all_heads, _ = qkv.shape
+    _, _, head_stride, last_stride = qkv.stride()
+    if (last_stride != 1 or (all_heads > 1 and head_stride != HEAD_DIM)) and qkv.numel():
         raise RuntimeError("the heads of a token of qkv must be contiguous")
-    _check_tensors((("cos", cos), ("sin", sin)), torch.float32, qkv.device)
+    index = qkv.get_device()
+    if not (_plain(cos, torch.float32, index) and _plain(sin, torch.float32, index)):
+        _check_tensors((("cos", cos), ("sin", sin)), torch.float32, qkv.device)
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise RuntimeError("cos and sin must have the same shape (positions, rotary_dim / 2)")
-    rotary = 2 * cos.shape[1]
+    table_rows, pairs = cos.shape
+    rotary = 2 * pairs
     if rotary == 0 or rotary > HEAD_DIM or rotary % 16 != 0:
         raise RuntimeError(f"rotary_dim must be a multiple of 16 up to {HEAD_DIM}")
     if (q_weight is None) != (k_weight is None):
         raise RuntimeError("q_weight and k_weight must be given together")
     if q_weight is not None:
-        if q_weight.dtype not in (torch.float32, torch.bfloat16):
+        dtype = q_weight.dtype
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise RuntimeError("q_weight must be fp32 or bf16")
-        _check_tensors((("q_weight", q_weight), ("k_weight", k_weight)), q_weight.dtype, qkv.device)
-        if tuple(q_weight.shape) != (HEAD_DIM,) or tuple(k_weight.shape) != (HEAD_DIM,):
+        if not (_plain(q_weight, dtype, index) and _plain(k_weight, dtype, index)):
+            _check_tensors((("q_weight", q_weight), ("k_weight", k_weight)), dtype, qkv.device)
+        if q_weight.dim() != 1 or q_weight.shape != k_weight.shape or q_weight.numel() != HEAD_DIM:
             raise RuntimeError(f"q_weight and k_weight must have shape ({HEAD_DIM},)")
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
@@ -281,25 +309,25 @@ def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, pos
             raise RuntimeError("sections need positions")
         section_array = (ctypes.c_int * axes)(*sections)
     if positions is None:
-        if seq > cos.shape[0]:
+        if seq > table_rows:
             raise RuntimeError("cos and sin have fewer rows than the sequence has tokens")
     else:
-        if not positions.is_cuda or positions.device != qkv.device:
+        if not positions.is_cuda or positions.get_device() != index:
             raise RuntimeError("positions must be on the device of qkv")
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype is not torch.int32 and positions.dtype is not torch.int64:
             raise RuntimeError("positions must be int32 or int64")
-        shape = tuple(positions.shape) if sections is None else tuple(positions.shape[1:])
-        if shape not in ((seq,), (batch, seq)) or (sections is not None and positions.shape[0] != axes):
+        shape = positions.shape if sections is None else positions.shape[1:]
+        if shape != (batch, seq) and shape != (seq,) or (sections is not None and positions.shape[0] != axes):
             lead = "" if sections is None else "axes, "
             raise RuntimeError(f"positions must have shape ({lead}seq) or ({lead}batch, seq)")
-        if cos.shape[0] == 0 and positions.numel():
+        if table_rows == 0 and positions.numel():
             raise RuntimeError("cos and sin have no rows")
         at = positions.stride()
         strides = (at[0] if sections is not None else 0, at[-2] if len(shape) == 2 else 0, at[-1])
     args = [batch, seq, heads, kv_heads, HEAD_DIM,
             None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
             int(q_weight is not None and q_weight.dtype == torch.bfloat16), cos.data_ptr(), sin.data_ptr(),
-            cos.shape[0], rotary, 1 if interleaved else 0, None if positions is None else positions.data_ptr(),
+            table_rows, rotary, 1 if interleaved else 0, None if positions is None else positions.data_ptr(),
             int(positions is not None and positions.dtype == torch.int64), *strides, axes,
             None if section_array is None else ctypes.addressof(section_array), eps]
     return batch, seq, args, section_array
@@ -307,22 +335,24 @@ def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, pos
 
 def _qkv_strides(qkv) -> tuple[int, int]:
     """Batch and token stride (a dimension of one element has no stride to speak of)."""
-    return (qkv.stride(0) if qkv.shape[0] > 1 else 0), (qkv.stride(1) if qkv.shape[1] > 1 else 0)
+    (batch, seq, _, _), (at, by, _, _) = qkv.shape, qkv.stride()
+    return (at if batch > 1 else 0), (by if seq > 1 else 0)
 
 
 def _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved):
     torch = _torch()
     batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
                                         interleaved)
-    q, k, v = (torch.empty((batch, n, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
-               for n in (heads, kv_heads, kv_heads))
+    q = torch.empty((batch, heads, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
+    k = torch.empty((batch, kv_heads, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
+    v = torch.empty_like(k)
     if qkv.numel() == 0:
         return q, k, v
-    lib = b.load_library()
+    b.load_library()
     index = qkv.get_device()
     with _on(index):
-        code = lib.avo_b200_qkv_norm_rope(qkv.data_ptr(), *_qkv_strides(qkv), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                          *args, b.status_word(index).data_ptr(), b._raw_stream(index))
+        code = b.call_entry(2, qkv.data_ptr(), *_qkv_strides(qkv), q.data_ptr(), k.data_ptr(), v.data_ptr(), *args,
+                            b.status_address(index), b._raw_stream(index))
     del keep
     b._check(code, "avo_b200_qkv_norm_rope")
     return q, k, v
@@ -336,7 +366,10 @@ def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight
     arguments are the forward's.  dqkv is a new contiguous tensor of qkv's shape, the weight
     gradients are fp32 [128] (None without weights).  Equal inputs give equal bits."""
     torch = _torch()
-    _check_tensors((("dq", dq), ("dk", dk), ("dv", dv)), torch.bfloat16, qkv.device)
+    index = qkv.get_device()
+    if not (_plain(dq, torch.bfloat16, index) and _plain(dk, torch.bfloat16, index)
+            and _plain(dv, torch.bfloat16, index)):
+        _check_tensors((("dq", dq), ("dk", dk), ("dv", dv)), torch.bfloat16, qkv.device)
     if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape:
         raise RuntimeError("dq, dk and dv must have shape (batch, heads, seq, dim), dk and dv the same")
     heads, kv_heads = dq.shape[1], dk.shape[1]
@@ -345,18 +378,18 @@ def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight
     if tuple(dq.shape) != (batch, heads, seq, HEAD_DIM) or tuple(dk.shape) != (batch, kv_heads, seq, HEAD_DIM):
         raise RuntimeError("dq, dk and dv must match qkv's batch and sequence")
     dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-    lib = b.load_library()
+    b.load_library()
     index = qkv.get_device()
     with _on(index):
         weights, scratch, size = (None, None), None, 0
         if q_weight is not None:
-            weights = tuple(torch.empty(HEAD_DIM, dtype=torch.float32, device=qkv.device) for _ in range(2))
+            weights = tuple(torch.empty((2, HEAD_DIM), dtype=torch.float32, device=qkv.device).unbind())
             size = _rope_scratch_bytes(index)
             scratch = torch.empty(size, dtype=torch.uint8, device=qkv.device)
-        code = lib.avo_b200_qkv_norm_rope_bwd(
-            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), *_qkv_strides(qkv),
-            dqkv.data_ptr(), *(None if w is None else w.data_ptr() for w in weights), *args,
-            None if scratch is None else scratch.data_ptr(), size, b.status_word(index).data_ptr(),
+        code = b.call_entry(
+            3, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), *_qkv_strides(qkv), dqkv.data_ptr(),
+            None if q_weight is None else weights[0].data_ptr(), None if q_weight is None else weights[1].data_ptr(),
+            *args, None if scratch is None else scratch.data_ptr(), size, b.status_address(index),
             b._raw_stream(index))
     del keep
     b._check(code, "avo_b200_qkv_norm_rope_bwd")
@@ -429,7 +462,8 @@ def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=
     torch = _torch()
     sections = None if sections is None else tuple(int(n) for n in sections)
     heads, kv_heads, interleaved = int(num_heads), int(num_kv_heads), bool(interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved)
         with _on(qkv.get_device()):
             _refuse_capture("qkv_norm_rope")
