@@ -9,8 +9,6 @@
 namespace avo_b200 {
 namespace {
 
-constexpr int kBwdCtasPerSm = 4;  // CTAs of the backward kernel per multiprocessor
-
 // What both directions share: checks and fills everything but the in/out tensors.
 int fill(rope::RopeParams& p, const void* qkv, long long stride_b, long long stride_s, int batch, int seq, int heads,
          int kv_heads, int head_dim, const void* q_weight, const void* k_weight, int weight_bf16, const float* cos,
@@ -76,7 +74,9 @@ void split_heads(rope::RopeParams& p, int sms) {
   p.heads_per_task = per;
   p.segs_q = segs(p.heads, per);
   p.segs_kv = segs(p.kv_heads, per);
-  p.tasks = pairs * (p.segs_q + 2 * p.segs_kv);
+  p.q_tasks = pairs * p.segs_q;
+  p.k_tasks = pairs * p.segs_kv;
+  p.tasks = p.q_tasks + 2 * p.k_tasks;
 }
 
 long long ctas_for(long long tasks) { return (tasks + rope::kWarps - 1) / rope::kWarps; }
@@ -125,7 +125,7 @@ extern "C" int avo_b200_qkv_norm_rope_bwd_workspace_size(size_t* bytes) {
   int sms = 0;
   const int rc = host::device(&sms);
   if (rc != AVO_B200_OK) return rc;
-  *bytes = static_cast<size_t>(sms) * kBwdCtasPerSm * 2 * rope::kRow * sizeof(float);
+  *bytes = static_cast<size_t>(sms) * rope::kBwdCtasPerSm * 2 * rope::kRow * sizeof(float);
   return AVO_B200_OK;
 }
 
@@ -167,7 +167,7 @@ extern "C" int avo_b200_qkv_norm_rope_bwd(const void* dq, const void* dk, const 
   p.dqkv = static_cast<__nv_bfloat16*>(dqkv);
   split_heads(p, sms);
   long long ctas = ctas_for(p.tasks);
-  const long long most = static_cast<long long>(sms) * kBwdCtasPerSm;
+  const long long most = static_cast<long long>(sms) * rope::kBwdCtasPerSm;
   if (ctas > most) ctas = most;
   if (norm && (workspace == nullptr || !host::aligned(workspace, 16) ||
                workspace_bytes < static_cast<size_t>(ctas) * 2 * rope::kRow * sizeof(float)))

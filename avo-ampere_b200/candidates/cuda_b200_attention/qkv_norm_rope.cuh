@@ -14,11 +14,11 @@
 // p(dy) sin) and passes the norm: dw = sum g x_hat, dx = r (g w - x_hat mean(g w x_hat)); r
 // is recomputed from x, nothing is saved.
 //
-// Both directions move bytes: 16 lanes hold one head's row (16 bytes a lane, so a row is one
-// 256-byte access), a half-warp owns one token and walks `heads_per_task` of its heads, four
-// rows in flight at a time.  Everything is fp32 between the load and one rounding to bf16.
-// The weights' gradients are summed per thread, then per CTA, then over CTAs by a second
-// kernel, each in a fixed order: equal inputs give equal bits.
+// Both directions move bytes: 16 lanes hold one head's row (8 values a lane, both halves of its
+// pairs among them, so a rotation needs no other lane), a half-warp owns one token and walks
+// `heads_per_task` of its heads, four rows in flight at a time.  Everything is fp32 between
+// the load and one rounding to bf16.  The weights' gradients are summed per thread, then per
+// CTA, then over CTAs by a second kernel, each in a fixed order: equal inputs give equal bits.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -33,6 +33,8 @@ constexpr int kThreadsRope = 128;
 constexpr int kWarps = kThreadsRope / 32;
 constexpr int kMaxAxes = 4;
 constexpr int kUnroll = 4;              // rows in flight per half-warp
+constexpr int kFwdCtasPerSm = 8;        // resident CTAs (bounds the registers)
+constexpr int kBwdCtasPerSm = 4;
 constexpr int kStatusPosition = 4;      // a position lies outside the table
 
 struct RopeParams {
@@ -59,31 +61,70 @@ struct RopeParams {
   float eps;
   int* status;
   int heads_per_task;
-  int segs_q, segs_kv;                  // tasks per token pair: query, key (and value) heads
-  long long tasks;
+  int segs_q, segs_kv;                  // tasks per token pair: query heads, key (or value) heads
+  long long q_tasks, k_tasks, tasks;    // query tasks, then key tasks, then value tasks
 };
 
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-__device__ __forceinline__ void load_weights(const void* w, int bf16, int col, float (&out)[8]) {
-  if (bf16) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + col));
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out[2 * i] = lo_f(u[i]);
-      out[2 * i + 1] = hi_f(u[i]);
-    }
+// The 8 columns of lane l: two groups of 4.  Pairs (f, f + rot/2): 4 first halves and their 4
+// second halves.  Interleaved pairs, and columns past the rotated part: 8 in a row.
+struct Columns {
+  int lo, hi;
+  bool turned;
+};
+template <bool kInterleaved>
+__device__ __forceinline__ Columns columns_of(int l, int rot) {
+  const bool turned = l * 8 < rot;
+  if (kInterleaved || !turned) return {l * 8, l * 8 + 4, turned};
+  return {l * 4, (rot >> 1) + l * 4, true};
+}
+
+// A row's 8 values of this lane as four bf16 pairs.
+template <bool kInterleaved>
+__device__ __forceinline__ uint4 load_row(const __nv_bfloat16* row, const Columns& c) {
+  if (kInterleaved) return __ldg(reinterpret_cast<const uint4*>(row + c.lo));
+  const uint2 a = __ldg(reinterpret_cast<const uint2*>(row + c.lo));
+  const uint2 b = __ldg(reinterpret_cast<const uint2*>(row + c.hi));
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+template <bool kInterleaved>
+__device__ __forceinline__ void store_row(__nv_bfloat16* row, const Columns& c, uint4 v) {
+  if (kInterleaved) {
+    *reinterpret_cast<uint4*>(row + c.lo) = v;
   } else {
-    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(w) + col);
-    const float4 a = __ldg(f), b = __ldg(f + 1);
-    out[0] = a.x; out[1] = a.y; out[2] = a.z; out[3] = a.w;
-    out[4] = b.x; out[5] = b.y; out[6] = b.z; out[7] = b.w;
+    *reinterpret_cast<uint2*>(row + c.lo) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(row + c.hi) = make_uint2(v.z, v.w);
   }
 }
 
-// One task: a pair of tokens (one per half-warp) and a run of heads of one kind.
+// Four values of a weight from column `col` (a multiple of 4).
+__device__ __forceinline__ void load_weight4(const void* w, int bf16, int col, float* out) {
+  if (bf16) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + col));
+    out[0] = lo_f(a.x);
+    out[1] = hi_f(a.x);
+    out[2] = lo_f(a.y);
+    out[3] = hi_f(a.y);
+  } else {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + col));
+    out[0] = a.x;
+    out[1] = a.y;
+    out[2] = a.z;
+    out[3] = a.w;
+  }
+}
+
+__device__ __forceinline__ void load_weights(const void* w, int bf16, const Columns& c, float (&out)[8]) {
+  load_weight4(w, bf16, c.lo, out);
+  load_weight4(w, bf16, c.hi, out + 4);
+}
+
+// One task: a pair of tokens (one per half-warp) and a run of their heads of one kind.  All
+// query tasks come first, then the key tasks, then the value tasks, so that the warps of a CTA
+// have equal work and a warp that walks many tasks changes kind twice at most.
 struct Task {
   int kind;       // 0 query, 1 key, 2 value
   int h0, h1;     // heads of that kind
@@ -94,22 +135,12 @@ struct Task {
 
 __device__ __forceinline__ Task decode(const RopeParams& p, long long task, int half) {
   Task t;
-  const int per = p.segs_q + 2 * p.segs_kv;
-  const long long pair = task / per;
-  int seg = static_cast<int>(task - pair * per);
-  int heads = p.heads;
-  t.kind = 0;
-  if (seg >= p.segs_q) {
-    seg -= p.segs_q;
-    heads = p.kv_heads;
-    t.kind = 1;
-    if (seg >= p.segs_kv) {
-      seg -= p.segs_kv;
-      t.kind = 2;
-    }
-  }
-  t.h0 = seg * p.heads_per_task;
-  t.h1 = min(heads, t.h0 + p.heads_per_task);
+  t.kind = task < p.q_tasks ? 0 : (task < p.q_tasks + p.k_tasks ? 1 : 2);
+  task -= t.kind == 0 ? 0 : (t.kind == 1 ? p.q_tasks : p.q_tasks + p.k_tasks);
+  const int segs = t.kind == 0 ? p.segs_q : p.segs_kv;
+  const long long pair = task / segs;
+  t.h0 = static_cast<int>(task - pair * segs) * p.heads_per_task;
+  t.h1 = min(t.kind == 0 ? p.heads : p.kv_heads, t.h0 + p.heads_per_task);
   const long long token = 2 * pair + half;
   t.valid = token < p.tokens;
   t.token = t.valid ? static_cast<int>(token) : p.tokens - 1;
@@ -118,11 +149,17 @@ __device__ __forceinline__ Task decode(const RopeParams& p, long long task, int 
   return t;
 }
 
+// First head of a kind in the projection, and its place in [batch, heads, seq, 128].
+__device__ __forceinline__ int first_head(const RopeParams& p, int kind) {
+  return kind == 0 ? 0 : (kind == 1 ? p.heads : p.heads + p.kv_heads);
+}
+__device__ __forceinline__ long long row_at(const RopeParams& p, const Task& t, int h) {
+  return ((static_cast<long long>(t.batch) * (t.kind == 0 ? p.heads : p.kv_heads) + h) * p.seq + t.s) * kRow;
+}
+
 // cos and sigma * sin of this lane's 8 columns (1 and 0 past the rotated part).
 template <bool kInterleaved>
 __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, int l, float (&c)[8], float (&s)[8]) {
-  const int half_lanes = p.rot >> 4;  // lanes per half of the rotated part
-  const int half_rot = p.rot >> 1;
   if (l * 8 >= p.rot) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -131,6 +168,7 @@ __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, in
     }
     return;
   }
+  const int half_rot = p.rot >> 1;
   long long row[kMaxAxes];
   bool bad = false;
 #pragma unroll
@@ -150,9 +188,8 @@ __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, in
     }
   }
   if (bad && t.valid && l == 0 && p.status != nullptr) atomicOr(p.status, kStatusPosition);
-  constexpr int kCols = kInterleaved ? 4 : 8;  // table columns this lane uses
-  const int col = kInterleaved ? l * 4 : (l < half_lanes ? l : l - half_lanes) * 8;
-  float cc[kCols], ss[kCols];
+  const int col = l * 4;  // this lane turns pairs col .. col + 3, table columns of the same index
+  float cc[4], ss[4];
   auto row_of = [&](int f) {
     long long r = row[0];
 #pragma unroll
@@ -160,18 +197,14 @@ __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, in
       if (a < p.axes && f >= p.end[a - 1]) r = row[a];
     return r;
   };
-  const long long first = row_of(col);
   if (p.axes == 1) {
-#pragma unroll
-    for (int i = 0; i < kCols; i += 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + first * half_rot + col + i));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + first * half_rot + col + i));
-      cc[i] = a.x; cc[i + 1] = a.y; cc[i + 2] = a.z; cc[i + 3] = a.w;
-      ss[i] = b.x; ss[i + 1] = b.y; ss[i + 2] = b.z; ss[i + 3] = b.w;
-    }
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row[0] * half_rot + col));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row[0] * half_rot + col));
+    cc[0] = a.x; cc[1] = a.y; cc[2] = a.z; cc[3] = a.w;
+    ss[0] = b.x; ss[1] = b.y; ss[2] = b.z; ss[3] = b.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const long long at = row_of(col + i) * half_rot + col + i;
       cc[i] = __ldg(p.cos + at);
       ss[i] = __ldg(p.sin + at);
@@ -180,22 +213,17 @@ __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, in
   const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int i = kInterleaved ? e / 2 : e;
-    const bool minus = kInterleaved ? (e & 1) == 0 : l < half_lanes;
+    const int i = kInterleaved ? e >> 1 : e & 3;
+    const bool minus = kInterleaved ? (e & 1) == 0 : e < 4;
     c[e] = bad ? nan : cc[i];
     s[e] = bad ? nan : (minus ? -ss[i] : ss[i]);
   }
 }
 
-// The other halves of this lane's 8 values (bf16 pairs).  Every lane of the warp calls it.
+// Index of the other half of value e of a lane.
 template <bool kInterleaved>
-__device__ __forceinline__ uint4 partner_of(uint4 x, int src_lane) {
-  if (kInterleaved) {
-    return make_uint4(__funnelshift_l(x.x, x.x, 16), __funnelshift_l(x.y, x.y, 16), __funnelshift_l(x.z, x.z, 16),
-                      __funnelshift_l(x.w, x.w, 16));
-  }
-  return make_uint4(__shfl_sync(0xffffffffu, x.x, src_lane), __shfl_sync(0xffffffffu, x.y, src_lane),
-                    __shfl_sync(0xffffffffu, x.z, src_lane), __shfl_sync(0xffffffffu, x.w, src_lane));
+__device__ __forceinline__ constexpr int other(int e) {
+  return kInterleaved ? e ^ 1 : e ^ 4;
 }
 
 __device__ __forceinline__ float half_sum(float v) {
@@ -204,167 +232,229 @@ __device__ __forceinline__ float half_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ void unpack8(uint4 x, float (&f)[8]) {
-  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = lo_f(u[i]);
-    f[2 * i + 1] = hi_f(u[i]);
+// The four packed fp32 pairs of a lane's values, and the pairs of their other halves.
+__device__ __forceinline__ void unpack4(uint4 x, uint64_t (&f)[4]) {
+  f[0] = f2_pack(lo_f(x.x), hi_f(x.x));
+  f[1] = f2_pack(lo_f(x.y), hi_f(x.y));
+  f[2] = f2_pack(lo_f(x.z), hi_f(x.z));
+  f[3] = f2_pack(lo_f(x.w), hi_f(x.w));
+}
+template <bool kInterleaved>
+__device__ __forceinline__ void others4(uint4 x, const uint64_t (&f)[4], uint64_t (&g)[4]) {
+  if (kInterleaved) {
+    g[0] = f2_pack(hi_f(x.x), lo_f(x.x));
+    g[1] = f2_pack(hi_f(x.y), lo_f(x.y));
+    g[2] = f2_pack(hi_f(x.z), lo_f(x.z));
+    g[3] = f2_pack(hi_f(x.w), lo_f(x.w));
+  } else {
+    g[0] = f[2];
+    g[1] = f[3];
+    g[2] = f[0];
+    g[3] = f[1];
   }
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+__device__ __forceinline__ uint4 pack4(const uint64_t (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2_unpack(f[i], a, b);
+    w[i] = pack_bf16x2(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Lane of the half-warp that holds the other halves of this lane's columns.
-__device__ __forceinline__ int partner_lane(int l, int rot) {
-  const int h = rot >> 4;
-  return l < h ? l + h : (l < 2 * h ? l - h : l);
+__device__ __forceinline__ float sum2(const uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+// Sum over the row of u * v (packed pairs).
+__device__ __forceinline__ float row_dot(const uint64_t (&u)[4], const uint64_t (&v)[4]) {
+  uint64_t a = f2_mul(u[0], v[0]), b = f2_mul(u[1], v[1]);
+  a = f2_fma(u[2], v[2], a);
+  b = f2_fma(u[3], v[3], b);
+  return half_sum(sum2(f2_add(a, b)));
 }
 
 template <bool kInterleaved>
-__global__ void __launch_bounds__(kThreadsRope) qkv_norm_rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreadsRope, kFwdCtasPerSm)
+    qkv_norm_rope_kernel(const __grid_constant__ RopeParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, l = lane & 15, half = lane >> 4;
   const long long task = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   if (task >= p.tasks) return;
   const Task t = decode(p, task, half);
-  const int head_base = t.kind == 0 ? 0 : (t.kind == 1 ? p.heads : p.heads + p.kv_heads);
-  const int out_heads = t.kind == 0 ? p.heads : p.kv_heads;
-  __nv_bfloat16* const dst = t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v);
-  const __nv_bfloat16* const src = p.qkv + t.batch * p.stride_b + t.s * p.stride_s + l * 8;
-  auto out_row = [&](int h) {
-    return reinterpret_cast<uint4*>(dst + ((static_cast<long long>(t.batch) * out_heads + h) * p.seq + t.s) * kRow +
-                                    l * 8);
-  };
-  float a[8], b[8];
-  const bool norm = p.q_weight != nullptr;
-  const int src_lane = half * 16 + partner_lane(l, p.rot);
-  if (t.kind < 2) {
-    load_turn<kInterleaved>(p, t, l, a, b);
-    if (norm) {
-      float w[8], wp[8];
-      const void* weight = t.kind == 0 ? p.q_weight : p.k_weight;
-      load_weights(weight, p.weight_bf16, l * 8, w);
-      load_weights(weight, p.weight_bf16, kInterleaved ? l * 8 : partner_lane(l, p.rot) * 8, wp);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[e] *= w[e];
-        b[e] *= wp[kInterleaved ? e ^ 1 : e];
-      }
-    }
-  }
-  for (int h = t.h0; h < t.h1; h += kUnroll) {
-    uint4 x[kUnroll];
+  const Columns col = columns_of<kInterleaved>(l, p.rot);
+  const __nv_bfloat16* src =
+      p.qkv + t.batch * p.stride_b + t.s * p.stride_s + static_cast<long long>(first_head(p, t.kind) + t.h0) * kRow;
+  const long long step = static_cast<long long>(p.seq) * kRow;
+  __nv_bfloat16* dst = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
+  uint4 x[kUnroll];
+  int left = t.h1 - t.h0;
+  auto load = [&]() {
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i)
-      if (h + i < t.h1) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (head_base + h + i) * kRow));
+      if (i < left) x[i] = load_row<kInterleaved>(src + i * kRow, col);
+    src += kUnroll * kRow;
+  };
+  load();
+  if (t.kind == 2) {
+    for (; left > 0; left -= kUnroll, dst += kUnroll * step) {
+      if (left < t.h1 - t.h0) load();
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i)
+        if (i < left && t.valid) store_row<kInterleaved>(dst + i * step, col, x[i]);
+    }
+    return;
+  }
+  const bool norm = p.q_weight != nullptr;
+  uint64_t a[4], b[4];
+  {
+    float c[8], s[8];
+    load_turn<kInterleaved>(p, t, l, c, s);
+    if (norm) {
+      float w[8];
+      load_weights(t.kind == 0 ? p.q_weight : p.k_weight, p.weight_bf16, col, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] *= w[e];
+        s[e] *= col.turned ? w[other<kInterleaved>(e)] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = f2_pack(c[2 * i], c[2 * i + 1]);
+      b[i] = f2_pack(s[2 * i], s[2 * i + 1]);
+    }
+  }
+  for (; left > 0; left -= kUnroll, dst += kUnroll * step) {
+    if (left < t.h1 - t.h0) load();
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      if (h + i >= t.h1) break;
-      uint4 y = x[i];
-      if (t.kind < 2) {
-        float f[8], g[8];
-        unpack8(x[i], f);
-        unpack8(partner_of<kInterleaved>(x[i], src_lane), g);
-        float r = 1.f;
-        if (norm) {
-          float sq = 0.f;
+      if (i >= left) break;
+      uint64_t f[4], g[4];
+      unpack4(x[i], f);
+      others4<kInterleaved>(x[i], f, g);
+      const float r = norm ? rsqrtf(row_dot(f, f) * (1.f / kRow) + p.eps) : 1.f;
+      const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sq = fmaf(f[e], f[e], sq);
-          r = rsqrtf(half_sum(sq) * (1.f / kRow) + p.eps);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = r * fmaf(g[e], b[e], f[e] * a[e]);
-        y = pack8(f);
-      }
-      if (t.valid) *out_row(h + i) = y;
+      for (int e = 0; e < 4; ++e) f[e] = f2_mul(r2, f2_fma(g[e], b[e], f2_mul(f[e], a[e])));
+      if (t.valid) store_row<kInterleaved>(dst + i * step, col, pack4(f));
     }
   }
 }
 
 template <bool kInterleaved>
-__global__ void __launch_bounds__(kThreadsRope) qkv_norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
+    qkv_norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
   __shared__ float sums[kWarps][2][kRow];
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, l = lane & 15, half = lane >> 4, warp = threadIdx.x >> 5;
-  const int all_heads = p.heads + 2 * p.kv_heads;
   const bool norm = p.q_weight != nullptr;
-  const int src_lane = half * 16 + partner_lane(l, p.rot);
-  float dw[2][8];
+  const Columns col = columns_of<kInterleaved>(l, p.rot);
+  const long long step = static_cast<long long>(p.seq) * kRow;
+  uint64_t dw[4];  // weight gradient of the current kind
+  auto clear = [&]() {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.f;
+    for (int e = 0; e < 4; ++e) dw[e] = f2_pack(0.f, 0.f);
+  };
+  // Adds the two half-warps and leaves the warp's sum of `kind` in shared memory.
+  auto flush = [&](int kind) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v0, v1;
+      f2_unpack(dw[e >> 1], v0, v1);
+      float v = e & 1 ? v1 : v0;
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      if (half == 0) sums[warp][kind][(e < 4 ? col.lo : col.hi) + (e & 3)] = v;
+    }
+    clear();
+  };
+  clear();
+  int kind = 0;
   for (long long task = static_cast<long long>(blockIdx.x) * kWarps + warp; task < p.tasks;
        task += static_cast<long long>(gridDim.x) * kWarps) {
     const Task t = decode(p, task, half);
-    const int head_base = t.kind == 0 ? 0 : (t.kind == 1 ? p.heads : p.heads + p.kv_heads);
-    const int in_heads = t.kind == 0 ? p.heads : p.kv_heads;
-    const __nv_bfloat16* const dy = t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v);
-    const __nv_bfloat16* const src = p.qkv + t.batch * p.stride_b + t.s * p.stride_s + l * 8;
-    __nv_bfloat16* const dst = p.dqkv + static_cast<long long>(t.token) * all_heads * kRow + l * 8;
-    auto in_row = [&](int h) {
-      return reinterpret_cast<const uint4*>(
-          dy + ((static_cast<long long>(t.batch) * in_heads + h) * p.seq + t.s) * kRow + l * 8);
-    };
-    float c[8], s[8], w[8];
-    if (t.kind < 2) {
-      load_turn<kInterleaved>(p, t, l, c, s);
-      if (norm) load_weights(t.kind == 0 ? p.q_weight : p.k_weight, p.weight_bf16, l * 8, w);
-    }
-    for (int h = t.h0; h < t.h1; h += kUnroll) {
-      uint4 d[kUnroll], x[kUnroll];
+    for (; kind < t.kind; ++kind)
+      if (norm && kind < 2) flush(kind);
+    const int h_at = first_head(p, t.kind) + t.h0;
+    const __nv_bfloat16* src = p.qkv + t.batch * p.stride_b + t.s * p.stride_s + static_cast<long long>(h_at) * kRow;
+    __nv_bfloat16* dst =
+        p.dqkv + (static_cast<long long>(t.token) * (p.heads + 2 * p.kv_heads) + h_at) * kRow;
+    const __nv_bfloat16* in = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
+    int left = t.h1 - t.h0;
+    uint4 d[kUnroll], x[kUnroll];
+    auto load = [&]() {
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i)
-        if (h + i < t.h1) {
-          d[i] = __ldg(in_row(h + i));
-          if (t.kind < 2 && norm) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (head_base + h + i) * kRow));
+        if (i < left) {
+          d[i] = load_row<kInterleaved>(in + i * step, col);
+          if (t.kind < 2 && norm) x[i] = load_row<kInterleaved>(src + i * kRow, col);
         }
+      in += kUnroll * step;
+      src += kUnroll * kRow;
+    };
+    load();
+    if (t.kind == 2) {
+      for (; left > 0; left -= kUnroll, dst += kUnroll * kRow) {
+        if (left < t.h1 - t.h0) load();
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i)
+          if (i < left && t.valid) store_row<kInterleaved>(dst + i * kRow, col, d[i]);
+      }
+      continue;
+    }
+    uint64_t c2[4], s2[4], w2[4];
+    {
+      float c[8], s[8], w[8];
+      load_turn<kInterleaved>(p, t, l, c, s);
+      if (norm) load_weights(t.kind == 0 ? p.q_weight : p.k_weight, p.weight_bf16, col, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c2[i] = f2_pack(c[2 * i], c[2 * i + 1]);
+        s2[i] = f2_pack(-s[2 * i], -s[2 * i + 1]);
+        w2[i] = norm ? f2_pack(w[2 * i], w[2 * i + 1]) : 0;
+      }
+    }
+    for (; left > 0; left -= kUnroll, dst += kUnroll * kRow) {
+      if (left < t.h1 - t.h0) load();
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
-        if (h + i >= t.h1) break;
-        uint4 y = d[i];
-        if (t.kind < 2) {
-          float g[8], o[8];
-          unpack8(d[i], g);
-          unpack8(partner_of<kInterleaved>(d[i], src_lane), o);
+        if (i >= left) break;
+        uint64_t g[4], o[4], turned[4];
+        unpack4(d[i], g);
+        others4<kInterleaved>(d[i], g, o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = fmaf(-o[e], s[e], g[e] * c[e]);
-          if (norm) {
-            float f[8];
-            unpack8(x[i], f);
-            float sq = 0.f, dot = 0.f;
+        for (int e = 0; e < 4; ++e) turned[e] = f2_fma(o[e], s2[e], f2_mul(g[e], c2[e]));
+        if (norm) {
+          uint64_t f[4], gw[4];
+          unpack4(x[i], f);
+          const float r = rsqrtf(row_dot(f, f) * (1.f / kRow) + p.eps);
+          const uint64_t r2 = f2_pack(r, r);
+          const float live = t.valid ? 1.f : 0.f;
+          const uint64_t live2 = f2_pack(live, live);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              sq = fmaf(f[e], f[e], sq);
-              dot = fmaf(g[e] * w[e], f[e], dot);
-            }
-            const float r = rsqrtf(half_sum(sq) * (1.f / kRow) + p.eps);
-            const float m = half_sum(dot) * (1.f / kRow) * r;  // mean of g w x_hat
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float xh = f[e] * r;
-              const float gx = t.valid ? g[e] * xh : 0.f;
-              if (t.kind == 0) dw[0][e] += gx; else dw[1][e] += gx;
-              g[e] = r * fmaf(-xh, m, g[e] * w[e]);
-            }
+          for (int e = 0; e < 4; ++e) {
+            f[e] = f2_mul(f[e], r2);  // x_hat
+            gw[e] = f2_mul(turned[e], w2[e]);
+            dw[e] = f2_fma(f2_mul(turned[e], live2), f[e], dw[e]);
           }
-          y = pack8(g);
+          const float m = row_dot(gw, f) * (-1.f / kRow);  // -mean of g w x_hat
+          const uint64_t m2 = f2_pack(m, m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) turned[e] = f2_mul(r2, f2_fma(f[e], m2, gw[e]));
         }
-        if (t.valid) *reinterpret_cast<uint4*>(dst + (head_base + h + i) * kRow) = y;
+        if (t.valid) store_row<kInterleaved>(dst + i * kRow, col, pack4(turned));
       }
     }
   }
   if (!norm) return;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = dw[k][e] + __shfl_xor_sync(0xffffffffu, dw[k][e], 16);
-      if (half == 0) sums[warp][k][l * 8 + e] = v;
-    }
+  for (; kind < 2; ++kind) flush(kind);
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * kRow; i += kThreadsRope) {
     float v = 0.f;
