@@ -1,5 +1,6 @@
 // C-ABI entry points of the attention gradient (declared in include/avo_b200_attn.h): argument checks, tensor maps
 // and the three launches of attn_bwd.cuh.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -63,8 +64,86 @@ void fold_group(int& heads, int kv_heads, int& seq_q, int seq_kv, int& causal) {
   heads = kv_heads;
 }
 
-size_t stats_bytes(int batch, int heads, int seq_q) {
-  return static_cast<size_t>(batch) * heads * tiles_of(seq_q) * bwd::kStatBytes;
+// What a call runs, from its sizes alone (of a B200's 148 multiprocessors, so that neither the
+// scratch nor the results depend on the device that happens to be current).
+struct Sizes {
+  int q_heads, kv_heads, group;  // batch * heads
+  int seq_q, seq_kv, nq, nkv;
+  int causal, offset;
+  int split_kv, split_q;         // pieces per item of the dK/dV and of the dQ pass
+  size_t part_kv, part_q;        // bytes of one gradient's partial sums (dK or dV; dQ)
+};
+constexpr int kPlanSms = 148;
+
+// Pieces per item of a pass with `items` items of `longest` streamed tiles at most and `total`
+// tiles in all, whose join moves `bytes` per piece.  In microseconds: about `tile_us` for a
+// tile and three tiles' time for a unit's start and end; the join, about 4 and its bytes at
+// 4 TB/s.  One piece unless more win a tenth.
+int choose_split(double items, double longest, double total, double tile_us, double bytes) {
+  int best = 1;
+  double best_us = 0.0;
+  // (32 pieces keep every product of a tile count and a piece within 32 bits.)
+  if (longest * 32 > INT_MAX || items * 32 > INT_MAX) return 1;
+  for (int s = 1; s <= 32 && s <= longest; ++s) {
+    const double load = std::max(std::ceil(longest / s) + 3.0, total / kPlanSms + 3.0 * std::ceil(items * s / kPlanSms));
+    const double us = load * tile_us + (s > 1 ? 4.0 + s * bytes / 2e6 : 0.0);
+    if (s == 1 || us < (best == 1 ? 0.9 : 1.0) * best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
+Sizes sizes_of(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal) {
+  Sizes z{};
+  fold_group(heads, kv_heads, seq_q, seq_kv, causal);
+  z.q_heads = batch * heads;
+  z.kv_heads = batch * kv_heads;
+  z.group = heads / kv_heads;
+  z.seq_q = seq_q;
+  z.seq_kv = seq_kv;
+  z.nq = tiles_of(seq_q);
+  z.nkv = tiles_of(seq_kv);
+  z.causal = causal ? 1 : 0;
+  z.offset = causal ? seq_kv - seq_q : 0;
+  z.part_kv = static_cast<size_t>(z.kv_heads) * seq_kv * kHeadDim * sizeof(float);
+  z.part_q = static_cast<size_t>(z.q_heads) * seq_q * kHeadDim * sizeof(float);
+  if (z.part_kv == 0 || z.part_q == 0) {
+    z.split_kv = z.split_q = 1;
+    return z;
+  }
+  // Tiles that some row needs, of nq * nkv per query head: with a mask, about the visible pairs
+  // and half of the diagonal's tiles.
+  double pairs = static_cast<double>(z.nq) * z.nkv;
+  if (z.causal) {
+    const double rows = std::min(seq_q, seq_kv);  // rows that see a key
+    const double seen = rows * std::max(0, seq_kv - seq_q) + rows * (rows + 1.0) / 2.0;
+    pairs = std::min(pairs, seen / (kTile * kTile) + 0.5 * tiles_of(std::min(seq_q, seq_kv)));
+  }
+  const double kv_items = static_cast<double>(z.kv_heads) * z.nkv, q_items = static_cast<double>(z.q_heads) * z.nq;
+  const double total = pairs * z.q_heads;
+  z.split_kv = choose_split(kv_items, static_cast<double>(z.group) * z.nq, total, 1.35, 2.0 * z.part_kv);
+  z.split_q = choose_split(q_items, z.nkv, total, 1.0, static_cast<double>(z.part_q));
+  return z;
+}
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+void set_items(bwd::BwdParams& p, int heads, int tiles, int split) {
+  p.split = static_cast<uint32_t>(split);
+  p.split_magic = ~0ull / p.split + 1;  // unused for 1
+  p.item_count = static_cast<uint32_t>(heads) * static_cast<uint32_t>(tiles) * p.split;
+  p.item_div = static_cast<uint32_t>(p.causal ? heads : tiles);
+  p.item_magic = ~0ull / p.item_div + 1;
+}
+
+size_t stats_bytes(const Sizes& z) {
+  return round256(static_cast<size_t>(z.q_heads) * z.nq * bwd::kStatBytes);
+}
+
+size_t scratch_bytes(const Sizes& z) {
+  return stats_bytes(z) + (z.split_kv > 1 ? 2 * z.split_kv * z.part_kv : 0) + (z.split_q > 1 ? z.split_q * z.part_q : 0);
 }
 
 int zero(void* p, size_t bytes, cudaStream_t st) {
@@ -81,9 +160,9 @@ int zero(void* p, size_t bytes, cudaStream_t st) {
 using namespace avo_b200;
 
 extern "C" int avo_b200_attn_bwd_workspace_size(int batch, int heads, int kv_heads, int seq_q, int seq_kv,
-                                                size_t* bytes) {
+                                                int causal, size_t* bytes) {
   if (bytes == nullptr || !sizes_ok(batch, heads, kv_heads, seq_q, seq_kv)) return AVO_B200_EINVAL;
-  *bytes = stats_bytes(batch, heads, seq_q);  // not less than with the group folded
+  *bytes = scratch_bytes(sizes_of(batch, heads, kv_heads, seq_q, seq_kv, causal));
   return AVO_B200_OK;
 }
 
@@ -94,11 +173,8 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   if (head_dim != kHeadDim || !sizes_ok(batch, heads, kv_heads, seq_q, seq_kv)) return AVO_B200_EINVAL;
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return AVO_B200_EINVAL;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const size_t wanted = stats_bytes(batch, heads, seq_q);
-  fold_group(heads, kv_heads, seq_q, seq_kv, causal);
-  const int q_heads = batch * heads, kv_all = batch * kv_heads;
-  const size_t q_bytes = static_cast<size_t>(q_heads) * seq_q * kHeadDim * 2;
-  const size_t kv_bytes = static_cast<size_t>(kv_all) * seq_kv * kHeadDim * 2;
+  const Sizes z = sizes_of(batch, heads, kv_heads, seq_q, seq_kv, causal);
+  const size_t q_bytes = z.part_q / 2, kv_bytes = z.part_kv / 2;
   if (q_bytes == 0 || kv_bytes == 0) {
     // Nothing attends to anything: whichever gradients exist are zero.
     int rc = zero(dq, q_bytes, st);
@@ -113,59 +189,85 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   for (void* p : grads)
     if (p == nullptr || !host::aligned(p, 32)) return AVO_B200_EINVAL;
   if (lse == nullptr || !host::aligned(lse, 4)) return AVO_B200_EINVAL;
-  if (workspace == nullptr || !host::aligned(workspace, 256) || workspace_bytes < wanted)
+  if (workspace == nullptr || !host::aligned(workspace, 256) || workspace_bytes < scratch_bytes(z))
     return AVO_B200_EINVAL;
 
   int sms = 0;
   int rc = prepare_bwd(&sms);
   if (rc != AVO_B200_OK) return rc;
   alignas(64) CUtensorMap tq, tk, tv, tdo;
-  if ((rc = host::encode(&tq, q, seq_q, q_heads)) != AVO_B200_OK) return rc;
-  if ((rc = host::encode(&tdo, dout, seq_q, q_heads)) != AVO_B200_OK) return rc;
-  if ((rc = host::encode(&tk, k, seq_kv, kv_all)) != AVO_B200_OK) return rc;
-  if ((rc = host::encode(&tv, v, seq_kv, kv_all)) != AVO_B200_OK) return rc;
+  if ((rc = host::encode(&tq, q, z.seq_q, z.q_heads)) != AVO_B200_OK) return rc;
+  if ((rc = host::encode(&tdo, dout, z.seq_q, z.q_heads)) != AVO_B200_OK) return rc;
+  if ((rc = host::encode(&tk, k, z.seq_kv, z.kv_heads)) != AVO_B200_OK) return rc;
+  if ((rc = host::encode(&tv, v, z.seq_kv, z.kv_heads)) != AVO_B200_OK) return rc;
 
   bwd::BwdParams p{};
   p.stats = static_cast<const float*>(workspace);
   p.status = status_dev;
   p.watchdog_ns = host::watchdog_limit();
-  p.seq_q = seq_q;
-  p.seq_kv = seq_kv;
-  p.nq = tiles_of(seq_q);
-  p.nkv = tiles_of(seq_kv);
-  p.q_heads = q_heads;
-  p.kv_heads = kv_all;
-  p.group = heads / kv_heads;
-  p.causal = causal ? 1 : 0;
-  p.offset = causal ? seq_kv - seq_q : 0;
+  p.seq_q = z.seq_q;
+  p.seq_kv = z.seq_kv;
+  p.nq = z.nq;
+  p.nkv = z.nkv;
+  p.q_heads = z.q_heads;
+  p.kv_heads = z.kv_heads;
+  p.group = z.group;
+  p.causal = z.causal;
+  p.offset = z.offset;
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.test_skip_load = host::skip_load();
+  float* const part_dk = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(z));
+  float* const part_dv = part_dk + (z.split_kv > 1 ? z.split_kv * z.part_kv / sizeof(float) : 0);
+  float* const part_dq = part_dv + (z.split_kv > 1 ? z.split_kv * z.part_kv / sizeof(float) : 0);
 
-  const long long kv_items = static_cast<long long>(kv_all) * p.nkv, q_items = static_cast<long long>(q_heads) * p.nq;
+  const long long kv_units = static_cast<long long>(z.kv_heads) * z.nkv * z.split_kv;
+  const long long q_units = static_cast<long long>(z.q_heads) * z.nq * z.split_q;
   // Both passes at once where the dK/dV grid leaves multiprocessors idle from the start.
   // Measured on B200, at once against one after the other: B1 H4 S512 14.1 / 22.9 us, B1 H16
   // Hkv2 Q777 KV5003 137 / 144 us; but B1 H16 S4096 493 / 417 us: both passes slow down while
   // they share the chip.
-  p.overlap = kv_items < sms ? 1 : 0;
+  p.overlap = kv_units < sms ? 1 : 0;
 
-  const long long rows = static_cast<long long>(q_heads) * p.nq * kTile;
+  const long long rows = static_cast<long long>(z.q_heads) * p.nq * kTile;
   const long long blocks = rows / 16;
   if (blocks > INT_MAX) return AVO_B200_EINVAL;
   if (!host::launch_early(bwd::stats_kernel, static_cast<unsigned>(blocks), 256u, 0, st,
                           static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse,
-                          static_cast<float*>(workspace), rows, seq_q, p.nq))
+                          static_cast<float*>(workspace), rows, z.seq_q, p.nq))
     return AVO_B200_ELAUNCH;
+  set_items(p, z.kv_heads, z.nkv, z.split_kv);
   p.g1 = dk;
   p.g2 = dv;
-  if (!host::launch_early(bwd::attn_bwd_kernel<false>, static_cast<unsigned>(kv_items < sms ? kv_items : sms),
+  p.part1 = part_dk;
+  p.part2 = part_dv;
+  if (!host::launch_early(bwd::attn_bwd_kernel<false>, static_cast<unsigned>(kv_units < sms ? kv_units : sms),
                           bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tk, tv, tq, tdo, p))
     return AVO_B200_ELAUNCH;
+  set_items(p, z.q_heads, z.nq, z.split_q);
   p.g1 = dq;
   p.g2 = nullptr;
+  p.part1 = part_dq;
   p.x1 = q;
-  if (!host::launch_early(bwd::attn_bwd_kernel<true>, static_cast<unsigned>(q_items < sms ? q_items : sms),
+  if (!host::launch_early(bwd::attn_bwd_kernel<true>, static_cast<unsigned>(q_units < sms ? q_units : sms),
                           bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
     return AVO_B200_ELAUNCH;
+  if (z.split_kv > 1 || z.split_q > 1) {
+    bwd::JoinParams j{};
+    void* const out[3] = {dk, dv, dq};
+    const float* const part[3] = {part_dk, part_dv, part_dq};
+    long long groups = 0;
+    for (int g = 0; g < 3; ++g) {
+      const int split = g < 2 ? z.split_kv : z.split_q;
+      j.part[g] = part[g];
+      j.out[g] = static_cast<__nv_bfloat16*>(out[g]);
+      j.factor[g] = g == 1 ? 1.f : softmax_scale;
+      j.pieces[g] = static_cast<uint32_t>(split);
+      j.count[g] = split > 1 ? static_cast<long long>((g < 2 ? z.part_kv : z.part_q) / (8 * sizeof(float))) : 0;
+      groups += j.count[g];
+    }
+    if (!host::launch_early(bwd::join_kernel, static_cast<unsigned>((groups + 255) / 256), 256u, 0, st, j))
+      return AVO_B200_ELAUNCH;
+  }
   return cudaGetLastError() == cudaSuccess ? AVO_B200_OK : AVO_B200_ELAUNCH;
 }

@@ -174,16 +174,35 @@ struct BwdParams {
   float scale, scale_log2;
   int overlap;             // the two passes may run at the same time
   int test_skip_load;
+  // An item is a stationary tile; with split > 1 it is cut into that many pieces along the
+  // streamed tiles, each a unit of its own whose sums go to part1 / part2 in fp32
+  // ([split][heads][rows][128]), for join_kernel to add.
+  uint32_t split;
+  unsigned long long split_magic;
+  float* part1;
+  float* part2;
+  uint32_t item_count;     // units of this launch
+  uint32_t item_div;       // what an item's number is divided by: heads (causal) or tiles
+  unsigned long long item_magic;
 };
 
-// One CTA's items in order: (stationary tile of one head), waves over the grid in alternating
-// directions, causal items longest first.
+// w / div: with magic = ceil(2^64 / div) the high half of w * magic is exact for every 32-bit
+// w (the excess of magic is below 1, its product below 2^-32 of a step).
+__device__ __forceinline__ uint32_t div_by(uint32_t w, uint32_t div, unsigned long long magic) {
+  return div == 1 ? w : static_cast<uint32_t>(__umul64hi(w, magic));
+}
+
+// One CTA's units in order (a stationary tile of one head, or a piece of its work): waves over
+// the grid in alternating directions, causal items longest first.
 template <bool kDq>
 struct Items {
   const BwdParams& p;
-  int r = 0;
+  uint32_t r = 0;
   int head, tile;  // stationary head and tile
-  int t0, n;       // first streamed tile, tiles in all (dK/dV: over the whole group of heads)
+  int t0;          // first streamed tile that the item needs
+  int n;           // streamed tiles of this unit (dK/dV: over the whole group of heads)
+  int skip;        // of the item's tiles, those of earlier pieces
+  int piece;
   __device__ explicit Items(const BwdParams& params) : p(params) {}
   // The next item that has tiles.
   __device__ bool next_busy() {
@@ -193,38 +212,42 @@ struct Items {
     return true;
   }
   __device__ bool next() {
-    const int heads = kDq ? p.q_heads : p.kv_heads;
-    const int tiles = kDq ? p.nq : p.nkv;
-    const int count = heads * tiles;
-    const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+    const uint32_t grid = gridDim.x, cta = blockIdx.x;
     while (true) {
-      const long long base = static_cast<long long>(r) * grid;
-      if (base >= count) return false;
-      const long long w64 = base + ((r & 1) ? grid - 1 - cta : cta);
+      const unsigned long long base = static_cast<unsigned long long>(r) * grid;
+      if (base >= p.item_count) return false;
+      const uint32_t unit = static_cast<uint32_t>(base) + ((r & 1) ? grid - 1 - cta : cta);
       ++r;
-      if (w64 >= count) continue;
-      const int w = static_cast<int>(w64);
+      if (unit >= p.item_count) continue;
+      const uint32_t w = div_by(unit, p.split, p.split_magic);
+      piece = static_cast<int>(unit - w * p.split);
+      const uint32_t quotient = div_by(w, p.item_div, p.item_magic);
+      const int rest = static_cast<int>(w - quotient * p.item_div);
       if (p.causal) {
-        head = w % heads;
-        tile = kDq ? tiles - 1 - w / heads : w / heads;
+        head = rest;
+        tile = kDq ? p.nq - 1 - static_cast<int>(quotient) : static_cast<int>(quotient);
       } else {
-        head = w / tiles;
-        tile = w % tiles;
+        head = static_cast<int>(quotient);
+        tile = rest;
       }
+      t0 = 0;
       if (kDq) {
-        t0 = 0;
         n = p.nkv;
         if (p.causal) {
-          const int q_end = min(tile * kTile + kTile, p.seq_q);
-          const int last = q_end - 1 + p.offset;  // last key any row sees
-          n = last < 0 ? 0 : min(p.nkv, last / kTile + 1);
+          const int end = min(tile * kTile + kTile, p.seq_q) + p.offset;  // keys the last row sees
+          n = min(p.nkv, (max(end, 0) + kTile - 1) >> 7);
         }
       } else {
-        t0 = 0;
-        if (p.causal) t0 = min(max(0, tile * kTile - p.offset) / kTile, p.nq);
-        // A key tile past the last query's reach: max(0, k0 - offset) >= seq_q.
+        // The first query that sees the tile's first key; past the last query: no tiles.
+        if (p.causal) t0 = min(max(0, tile * kTile - p.offset) >> 7, p.nq);
         if (p.causal && tile * kTile - p.offset >= p.seq_q) t0 = p.nq;
         n = (p.nq - t0) * p.group;
+      }
+      skip = 0;
+      if (p.split > 1) {
+        const uint32_t all = static_cast<uint32_t>(n), pieces = p.split, at = static_cast<uint32_t>(piece);
+        skip = static_cast<int>(div_by(all * at, pieces, p.split_magic));
+        n = static_cast<int>(div_by(all * (at + 1), pieces, p.split_magic)) - skip;
       }
       return true;
     }
@@ -245,8 +268,14 @@ struct Tiles {
       if (!items.next_busy()) return false;
       left = items.n;
       first = true;
-      t = items.t0;
+      t = items.t0 + items.skip;
       y_head = kDq ? items.head / items.p.group : items.head * items.p.group;
+      if (!kDq && items.skip > 0) {
+        const int per_head = items.p.nq - items.t0;
+        const int heads = items.skip / per_head;
+        y_head += heads;
+        t -= heads * per_head;
+      }
     } else {
       ++t;
       if (!kDq && t == items.p.nq) {
@@ -622,10 +651,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int r = it.tile * kTile + row;
       const bool write = r < rows;
       const long long at = (static_cast<long long>(it.head) * rows + r) * kHeadDim;
+      const long long part_at =
+          ((static_cast<long long>(it.piece) * (kDq ? p.q_heads : p.kv_heads) + it.head) * rows + r) * kHeadDim;
       // dK/dV: dV (accumulator 2, complete first), then dK; dQ: accumulator 1 only.
 #pragma unroll 1
       for (int a = kDq ? 1 : 2; a >= 1; --a) {
         __nv_bfloat16* const dst = static_cast<__nv_bfloat16*>(a == 1 ? p.g1 : p.g2) + at;
+        float* const part = (a == 1 ? p.part1 : p.part2) + part_at;
         const float f = a == 1 ? p.scale : 1.f;
         const uint32_t acc = tmem + lane_off + (a == 1 ? kColAcc1 : kColAcc2);
         if (it.n > 0) {
@@ -650,7 +682,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             named_bar_arrive(a == 1 ? bar_acc1(done) : bar_acc2(done), kEpiThreads);
             ++acc_signals;
           }
-          if (write) {
+          if (write && p.split > 1) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              st_global_v8(part + c * 16 + e, o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+          } else if (write) {
             uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(u2f(o[2 * e]) * f, u2f(o[2 * e + 1]) * f);
@@ -721,8 +757,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int y_head = kDq ? ahead.head / p.group : ahead.head * p.group;
           if (!kDq) prefetch(&tm_x1, ahead.tile * kTile, ahead.head);
           prefetch(&tm_x2, ahead.tile * kTile, ahead.head);
-          prefetch(&tm_y1, ahead.t0 * kTile, y_head);
-          prefetch(&tm_y2, ahead.t0 * kTile, y_head);
+          prefetch(&tm_y1, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
+          prefetch(&tm_y2, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
         }
         const int s1 = n % kY1, s2 = n % kY2;
         // Y1's last user is its tile's last MMA: dQ, or dK, which precedes the next tile's T2.
@@ -919,6 +955,36 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
   // The dQ launch is complete only when the dK/dV launch is (see above).
   if (kDq && p.overlap) grid_dependency_wait();
+}
+
+// The sums of split units: out = bf16(factor * (part[0] + part[1] + ...)), in this order, for
+// up to three gradients (dK, dV, dQ; count 0: not split).  8 values per thread.
+struct JoinParams {
+  const float* part[3];
+  __nv_bfloat16* out[3];
+  float factor[3];
+  uint32_t pieces[3];
+  long long count[3];    // groups of 8 values
+};
+
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinParams p) {
+  grid_dependency_wait();
+  long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  int g = 0;
+  while (g < 3 && i >= p.count[g]) i -= p.count[g++];
+  if (g == 3) return;
+  const float4* src = reinterpret_cast<const float4*>(p.part[g]) + 2 * i;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+  for (uint32_t k = 0; k < p.pieces[g]; ++k) {
+    const float4 c = __ldcg(src), d = __ldcg(src + 1);
+    src += 2 * p.count[g];
+    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+    b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+  }
+  const float f = p.factor[g];
+  reinterpret_cast<uint4*>(p.out[g])[i] = make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f),
+                                                     pack_bf16x2(b.x * f, b.y * f), pack_bf16x2(b.z * f, b.w * f));
 }
 
 // -LSE*log2(e) and -delta of every query row, padded to whole tiles: [heads][nq][2][128].

@@ -66,7 +66,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
     "avo_b200_attn_bwd_workspace_size": (
         _c_int,
-        [_c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
+        [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
     ),
     "avo_b200_attn_bwd": (
         _c_int,

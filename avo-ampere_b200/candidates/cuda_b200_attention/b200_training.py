@@ -208,10 +208,10 @@ def grouped_attention(q, k, v, causal: bool, *, softmax_scale: float | None = No
 
 
 @functools.lru_cache(maxsize=256)
-def _backward_scratch_bytes(batch: int, heads: int, kv_heads: int, seq_q: int, seq_kv: int) -> int:
+def _backward_scratch_bytes(batch: int, heads: int, kv_heads: int, seq_q: int, seq_kv: int, causal: bool) -> int:
     """Scratch of the backward for these sizes."""
     size = ctypes.c_size_t(0)
-    b._check(b.load_library().avo_b200_attn_bwd_workspace_size(batch, heads, kv_heads, seq_q, seq_kv,
+    b._check(b.load_library().avo_b200_attn_bwd_workspace_size(batch, heads, kv_heads, seq_q, seq_kv, int(causal),
                                                                ctypes.byref(size)),
              "avo_b200_attn_bwd_workspace_size")
     return size.value
@@ -246,7 +246,7 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
     grads = (torch.empty_like(q) if dq is None else dq, torch.empty_like(k) if dk is None else dk,
              torch.empty_like(v) if dv is None else dv)
     with _on(index):
-        size = _backward_scratch_bytes(batch, heads, kv_heads, seq_q, seq_kv)
+        size = _backward_scratch_bytes(batch, heads, kv_heads, seq_q, seq_kv, bool(causal))
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         code = b.call_entry(
             1, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),

@@ -41,6 +41,9 @@ CASES = [
     (1, 6, 1, 1024, 129, False),
     (1, 16, 2, 1, 3000, True),    # one token of a long context, eight heads to a key
     (2, 9, 3, 5, 1111, False),
+    (1, 1, 1, 3000, 3000, True),     # one head: both passes split along the sequence
+    (1, 8, 1, 1500, 1200, True),
+    (1, 4, 2, 130, 6000, False),
 ]
 
 

@@ -10,7 +10,7 @@ FAKE = 0x10000
 
 def _bwd(lib, **over):
     a = dict(dout=FAKE, q=FAKE, k=FAKE, v=FAKE, o=FAKE, lse=FAKE, dq=FAKE, dk=FAKE, dv=FAKE, batch=1, heads=4,
-             kv_heads=2, seq_q=64, seq_kv=64, head_dim=128, causal=0, scale=0.088, ws=FAKE, ws_bytes=1 << 20)
+             kv_heads=2, seq_q=64, seq_kv=64, head_dim=128, causal=0, scale=0.088, ws=FAKE, ws_bytes=1 << 24)
     assert set(over) <= set(a)
     a.update(over)
     return lib.avo_b200_attn_bwd(*a.values(), None, None)
@@ -34,11 +34,17 @@ def test_attention_backward_workspace_size(b200):
     lib = b200.load_library()
     size = ctypes.c_size_t(0)
     ask = lib.avo_b200_attn_bwd_workspace_size
-    assert ask(1, 4, 2, 64, 64, None) == INVALID
-    assert ask(1, 4, 3, 64, 64, ctypes.byref(size)) == INVALID
+    assert ask(1, 4, 2, 64, 64, 0, None) == INVALID
+    assert ask(1, 4, 3, 64, 64, 1, ctypes.byref(size)) == INVALID
     for batch, heads, seq in ((1, 4, 1), (2, 8, 128), (1, 3, 129), (3, 2, 1000)):
-        assert ask(batch, heads, 1, seq, 77, ctypes.byref(size)) == 0
-        assert size.value >= batch * heads * -(-seq // 128) * 1024
+        for causal in (0, 1):
+            assert ask(batch, heads, 1, seq, 77, causal, ctypes.byref(size)) == 0
+            assert size.value >= batch * -(-heads * seq // 128) * 1024
+    # A long sequence of one head is split along itself: partial sums in fp32.
+    assert ask(1, 1, 1, 4096, 4096, 0, ctypes.byref(size)) == 0
+    assert size.value > 2 * 4096 * 128 * 4
+    # The largest sizes are answered without a loop over them.
+    assert ask(1, 1, 1, 2**31 - 1000, 2**31 - 1000, 1, ctypes.byref(size)) == 0
 
 
 def test_grouped_forward_refusals(b200):
