@@ -293,12 +293,15 @@ __global__ void __launch_bounds__(kThreadsRope, kFwdCtasPerSm)
       p.qkv + t.batch * p.stride_b + t.s * p.stride_s + static_cast<long long>(first_head(p, t.kind) + t.h0) * kRow;
   const long long step = static_cast<long long>(p.seq) * kRow;
   __nv_bfloat16* dst = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
+  // Rows past the run compute on ones and are not stored: without branches the rows' sums
+  // (shuffles) overlap.
+  const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
   uint4 x[kUnroll];
   int left = t.h1 - t.h0;
   auto load = [&]() {
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i)
-      if (i < left) x[i] = load_row<kInterleaved>(src + i * kRow, col);
+      x[i] = i < left ? load_row<kInterleaved>(src + i * kRow, col) : ones;
     src += kUnroll * kRow;
   };
   load();
@@ -335,7 +338,6 @@ __global__ void __launch_bounds__(kThreadsRope, kFwdCtasPerSm)
     if (left < t.h1 - t.h0) load();
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      if (i >= left) break;
       uint64_t f[4], g[4];
       unpack4(x[i], f);
       others4<kInterleaved>(x[i], f, g);
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kThreadsRope, kFwdCtasPerSm)
       const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = f2_mul(r2, f2_fma(g[e], b[e], f2_mul(f[e], a[e])));
-      if (t.valid) store_row<kInterleaved>(dst + i * step, col, pack4(f));
+      if (i < left && t.valid) store_row<kInterleaved>(dst + i * step, col, pack4(f));
     }
   }
 }
@@ -388,14 +390,15 @@ __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
         p.dqkv + (static_cast<long long>(t.token) * (p.heads + 2 * p.kv_heads) + h_at) * kRow;
     const __nv_bfloat16* in = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
     int left = t.h1 - t.h0;
+    const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
     uint4 d[kUnroll], x[kUnroll];
     auto load = [&]() {
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
-        if (i < left) {
-          d[i] = load_row<kInterleaved>(in + i * step, col);
-          if (t.kind < 2 && norm) x[i] = load_row<kInterleaved>(src + i * kRow, col);
-        }
+      for (int i = 0; i < kUnroll; ++i) {
+        // (Rows past the run: a zero gradient on ones.)
+        d[i] = i < left ? load_row<kInterleaved>(in + i * step, col) : make_uint4(0u, 0u, 0u, 0u);
+        x[i] = i < left && t.kind < 2 && norm ? load_row<kInterleaved>(src + i * kRow, col) : ones;
+      }
       in += kUnroll * step;
       src += kUnroll * kRow;
     };
@@ -425,7 +428,6 @@ __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
       if (left < t.h1 - t.h0) load();
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
-        if (i >= left) break;
         uint64_t g[4], o[4], turned[4];
         unpack4(d[i], g);
         others4<kInterleaved>(d[i], g, o);
@@ -434,22 +436,23 @@ __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
         if (norm) {
           uint64_t f[4], gw[4];
           unpack4(x[i], f);
-          const float r = rsqrtf(row_dot(f, f) * (1.f / kRow) + p.eps);
-          const uint64_t r2 = f2_pack(r, r);
+          // The two sums of the row are taken side by side: mean(g w x_hat) = r mean(g w x).
+#pragma unroll
+          for (int e = 0; e < 4; ++e) gw[e] = f2_mul(turned[e], w2[e]);
+          const float sq = row_dot(f, f), dot = row_dot(gw, f);
+          const float r = rsqrtf(sq * (1.f / kRow) + p.eps);
+          const float m = -dot * (1.f / kRow) * r;
+          const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
           const float live = t.valid ? 1.f : 0.f;
           const uint64_t live2 = f2_pack(live, live);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             f[e] = f2_mul(f[e], r2);  // x_hat
-            gw[e] = f2_mul(turned[e], w2[e]);
             dw[e] = f2_fma(f2_mul(turned[e], live2), f[e], dw[e]);
+            turned[e] = f2_mul(r2, f2_fma(f[e], m2, gw[e]));
           }
-          const float m = row_dot(gw, f) * (-1.f / kRow);  // -mean of g w x_hat
-          const uint64_t m2 = f2_pack(m, m);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) turned[e] = f2_mul(r2, f2_fma(f[e], m2, gw[e]));
         }
-        if (t.valid) store_row<kInterleaved>(dst + i * kRow, col, pack4(turned));
+        if (i < left && t.valid) store_row<kInterleaved>(dst + i * kRow, col, pack4(turned));
       }
     }
   }
