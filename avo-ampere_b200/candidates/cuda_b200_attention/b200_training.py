@@ -457,11 +457,14 @@ def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=
     NaN and is reported by ``check_status()``.
 
     With gradients enabled and an input that requires them, the result is differentiable in
-    qkv and the weights (once); such a call cannot be captured in a CUDA graph: capture the
-    call under ``torch.no_grad()`` and ``qkv_norm_rope_backward``."""
+    qkv and the weights (once), not in the tables, which must not require gradients then.
+    Such a call cannot be captured in a CUDA graph: capture the call under
+    ``torch.no_grad()`` and ``qkv_norm_rope_backward``."""
     torch = _torch()
     sections = None if sections is None else tuple(int(n) for n in sections)
     heads, kv_heads, interleaved = int(num_heads), int(num_kv_heads), bool(interleaved)
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise RuntimeError("qkv_norm_rope has no gradient for cos and sin: detach them")
     if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved)

@@ -391,6 +391,11 @@ def test_refusals(b200, seed):
     for more, args, match in bad:
         with pytest.raises(RuntimeError, match=match):
             seed.qkv_norm_rope(*args, **{**plain_how, **more})
+    for table in ((cos.clone().requires_grad_(), sin), (cos, sin.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient for cos and sin"):
+            seed.qkv_norm_rope(qkv, 4, 2, *table, **plain_how, positions=ok)
+        with torch.no_grad():
+            seed.qkv_norm_rope(qkv, 4, 2, *table, **plain_how, positions=ok)
     with pytest.raises(RuntimeError, match="match qkv"):
         seed.qkv_norm_rope_backward(grads[0][:, :, :9].contiguous(), *grads[1:], qkv, cos, sin, **how)
     with pytest.raises(RuntimeError, match="dq must be contiguous"):
