@@ -8,9 +8,10 @@ checks that every schedule ends, that no named barrier keeps arrivals, and that 
 (X1, X2, the Y1 and Y2 slots, the statistics slots, T1, T2, dS, the accumulators) is read
 before it is written or overwritten before it is read.  Planted mistakes must be caught.
 
-The abort is modelled too: at a random step every mbarrier wait starts to fail at once, as
-after a watchdog expiry; the roles then keep their barrier rounds as the kernel does, and
-every schedule still has to end with no arrivals left.
+The abort is modelled too: from a random step on every mbarrier wait whose phase has not
+completed gives up, as after a watchdog expiry, while the others go on; the roles then keep
+their barrier rounds as the kernel does.  Every schedule still has to end with no arrivals
+left, and no buffer may have two copies in flight.
 """
 
 from __future__ import annotations
@@ -43,6 +44,13 @@ class BwdModel(Model):
 
     # ---- primitives
     def wait(self, name, k):
+        """Yields whether the phase completed: after an abort a wait that has not gives up."""
+        ready = super().wait(name, k)
+        return lambda: "done" if ready() else "gave up" if self.aborted else False
+
+    def landed(self, name, k):
+        """The waiter's wait.  After an abort it no longer matters what it answers: copies that
+        were never made leave its phases behind."""
         ready = super().wait(name, k)
         return lambda: self.aborted or ready()
 
@@ -58,15 +66,18 @@ class BwdModel(Model):
             self.errors.append(text)
 
     def load(self, name, full, tag):
+        old = self.buf.get(name)
+        if old is not None and old[0] == "in flight":  # an abort does not excuse this
+            self.errors.append(f"{name}: a second copy ({tag}) while {old} is in flight")
         self.buf[name] = ("in flight", tag)
 
         def land():
-            self.buf[name] = tag
+            self.buf[name] = (tag,)
             self.complete(full)
         self.copies.append(land)
 
     def expect(self, who, name, tag):
-        if self.buf.get(name) != tag:
+        if self.buf.get(name) not in (tag, (tag,)):
             self.fail(f"{who}: {name} holds {self.buf.get(name)}, wanted {tag}")
 
     def t_full(self, which, u):
@@ -84,47 +95,38 @@ class BwdModel(Model):
         return 12 + (item % 2 if self.fault != "one_x1_barrier" else 0)
 
     # ---- loads
+    def reuse(self, fault, *wait):
+        """The wait before a buffer is loaded again; false after an abort."""
+        ok = True
+        if self.fault != fault:
+            ok = (yield wait[0]) == "done"
+        return ok and not self.aborted
+
     def producer(self):
         items = 0
         for n, (item, first, last) in enumerate(self.tiles):
             s1, s2 = n % self.y1, n % Y2
             if n >= self.y1:
-                if self.fault != "no_y1_wait":
-                    yield self.wait(f"Y1_EMPTY{s1}", n // self.y1 - 1) if self.dq else self.t_full(2, n - 2)
-                yield self.wait(f"Y1_FULL{s1}", n // self.y1 - 1)
-            if self.aborted:
-                return
+                done = self.wait(f"Y1_EMPTY{s1}", n // self.y1 - 1) if self.dq else self.t_full(2, n - 2)
+                if not (yield from self.reuse("no_y1_wait", done)):
+                    return
             self.load(f"Y1_{s1}", f"Y1_FULL{s1}", n)
             if first and not self.dq:
-                if items > 0:
-                    if self.fault != "no_x1_wait":
-                        yield self.t_full(1, n - 1)
-                    yield self.wait("X1_FULL", items - 1)
-                if self.aborted:
+                if items > 0 and not (yield from self.reuse("no_x1_wait", self.t_full(1, n - 1))):
                     return
                 self.load("X1", "X1_FULL", item)
             if n >= Y2:
-                if self.fault != "no_y2_wait":
-                    yield self.t_full(2, n - 2) if self.dq else self.wait(f"Y2_EMPTY{s2}", n // Y2 - 1)
-                yield self.wait(f"Y2_FULL{s2}", n // Y2 - 1)
-            if self.aborted:
-                return
+                done = self.t_full(2, n - 2) if self.dq else self.wait(f"Y2_EMPTY{s2}", n // Y2 - 1)
+                if not (yield from self.reuse("no_y2_wait", done)):
+                    return
             self.load(f"Y2_{s2}", f"Y2_FULL{s2}", n)
             if first:
-                if items > 0:
-                    if self.fault != "no_x2_wait":
-                        yield self.t_full(2, n - 1)
-                    yield self.wait("X2_FULL", items - 1)
-                if self.aborted:
+                if items > 0 and not (yield from self.reuse("no_x2_wait", self.t_full(2, n - 1))):
                     return
                 self.load("X2", "X2_FULL", item)
                 items += 1
             if not self.dq:
-                if n >= 2:
-                    if self.fault != "no_stat_wait":
-                        yield self.t_full(2, n - 1)
-                    yield self.wait(f"STAT{n % 2}", n // 2 - 1)
-                if self.aborted:
+                if n >= 2 and not (yield from self.reuse("no_stat_wait", self.t_full(2, n - 1))):
                     return
                 self.load(f"STAT_{n % 2}", f"STAT{n % 2}", n)
 
@@ -136,9 +138,9 @@ class BwdModel(Model):
             return
         item, first, last = self.tiles[n]
         if first and not (self.dq and which == 1):
-            yield self.wait(f"X{which}_FULL", self.busy.index(item))
+            yield self.landed(f"X{which}_FULL", self.busy.index(item))
         slots = self.y1 if which == 1 else Y2
-        yield self.wait(f"Y{which}_FULL{n % slots}", n // slots)
+        yield self.landed(f"Y{which}_FULL{n % slots}", n // slots)
 
     def waiter(self):
         self.seen = {1: 0, 2: 0}
@@ -296,10 +298,9 @@ class BwdModel(Model):
             if dead:
                 yield from self.rounds(n, 0)
                 continue
-            yield self.t_full(1, n)
-            if not self.dq:
-                yield self.wait(f"STAT{n % 2}", n // 2)
-            dead = self.aborted
+            dead = (yield self.t_full(1, n)) != "done"
+            if not self.dq and not dead:
+                dead = (yield self.wait(f"STAT{n % 2}", n // 2)) != "done"
             if dead:
                 yield from self.rounds(n, 0)
                 continue
@@ -314,8 +315,7 @@ class BwdModel(Model):
                     yield lambda: True
                     self.arrive(self.tile_bar(4 + half, n), warps=4)
             if self.fault != "no_t2_wait":
-                yield self.t_full(2, n)
-            dead = self.aborted
+                dead = (yield self.t_full(2, n)) != "done"
             if dead:
                 yield from self.rounds(n, 1)
                 continue
@@ -324,8 +324,7 @@ class BwdModel(Model):
                 yield lambda: True
                 self.arrive(self.tile_bar(5, n), warps=4)
                 if n > 0 and self.fault != "no_ds_wait":
-                    yield self.wait(f"Y1_EMPTY{(n - 1) % self.y1}", (n - 1) // self.y1)
-                dead = self.aborted
+                    dead = (yield self.wait(f"Y1_EMPTY{(n - 1) % self.y1}", (n - 1) // self.y1)) != "done"
                 if dead:
                     yield from self.rounds(n, 2)
                     continue
@@ -350,8 +349,7 @@ class BwdModel(Model):
             tiles += self.seq[item]
             if self.dq and k + 1 < len(self.busy):
                 if self.fault != "no_x1_wait":
-                    yield self.wait("X1_DONE", k)
-                ok = not self.aborted
+                    ok = (yield self.wait("X1_DONE", k)) == "done"
                 if not ok:
                     break
                 self.buf["X1"] = self.busy[k + 1]
@@ -359,8 +357,7 @@ class BwdModel(Model):
                 self.arrive(self.x1(k + 1), warps=4)
                 x_signals += 1
             for which in ([1] if self.dq else [2, 1]):
-                yield self.wait(f"ACC{which}", k)
-                ok = not self.aborted
+                ok = (yield self.wait(f"ACC{which}", k)) == "done"
                 if not ok:
                     break
                 self.expect(f"epilogue of item {item}", f"A{which}", ("sum", item, tiles - 1, 1))
@@ -408,7 +405,8 @@ class BwdModel(Model):
             steps += 1
             if self.abort_after is not None and steps > self.abort_after:
                 self.aborted = True
-            runnable = [r for r in range(len(roles)) if not done[r] and (ready[r] is None or ready[r]())]
+            answer = [True if ready[r] is None else not done[r] and ready[r]() for r in range(len(roles))]
+            runnable = [r for r in range(len(roles)) if not done[r] and answer[r]]
             n_async = len(self.copies) + (1 if self.pipe else 0)
             if not runnable and not n_async:
                 break
@@ -416,7 +414,7 @@ class BwdModel(Model):
             if pick < len(runnable):
                 r = runnable[pick]
                 try:
-                    ready[r] = next(roles[r])
+                    ready[r] = roles[r].send(None if ready[r] is None else answer[r])
                 except StopIteration:
                     done[r], ready[r] = True, None
             elif pick < len(runnable) + len(self.copies):
@@ -479,4 +477,4 @@ def test_mistakes_that_only_an_abort_shows_are_caught(fault, dqs):
     for dq in dqs:
         rnd = random.Random(4)
         assert any(errors_of(items, dq, trial, fault, rnd.randint(0, 300))
-                   for trial in range(300) for items in ([1, 1, 1, 1, 2], [5], [2, 1, 3])), (fault, dq)
+                   for trial in range(3000) for items in ([1, 1, 1, 1, 2], [5], [2, 1, 3])), (fault, dq)
