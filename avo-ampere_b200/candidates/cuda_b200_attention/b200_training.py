@@ -80,6 +80,12 @@ def _check_tensors(named, dtype, device=None) -> None:
             raise RuntimeError(f"{name} must be on {device}")
 
 
+def _overlap(a, b) -> bool:
+    """Whether two contiguous tensors share memory."""
+    at, by = a.data_ptr(), b.data_ptr()
+    return at < by + b.numel() * b.element_size() and by < at + a.numel() * a.element_size()
+
+
 def _attention_shape(q, k, v) -> tuple[int, int, int, int, int]:
     """(batch, heads, kv_heads, seq_q, seq_kv) of checked q, k, v."""
     bf16 = _torch().bfloat16
@@ -224,7 +230,8 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
     ``out`` and ``lse`` are what the forward (``grouped_attention``, or
     ``attention_with_lse`` for equal shapes) returned for the same inputs and scale.  dk and
     dv sum over the query heads that share a key/value head.  All tensors are contiguous;
-    the results go to ``dq``, ``dk``, ``dv`` where given.  The result does not depend on the
+    the results go to ``dq``, ``dk``, ``dv`` where given (which overlap no other tensor of the
+    call).  The result does not depend on the
     order in which the GPU runs the work: equal inputs give equal bits."""
     torch = _torch()
     batch, heads, kv_heads, seq_q, seq_kv = _attention_shape(q, k, v)
@@ -238,11 +245,13 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
         raise RuntimeError(f"{'out' if dout.shape == q.shape else 'dout'} must have the shape of q")
     if lse.shape != q.shape[:3]:
         raise RuntimeError("lse must have shape (batch, heads, seq)")
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t is not None:
-            _check_tensors(((name, t),), torch.bfloat16, q.device)
-            if t.shape != like.shape:
-                raise RuntimeError(f"{name} must have the shape of {name[1:]}")
+    given = [(name, t, like) for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)) if t is not None]
+    for i, (name, t, like) in enumerate(given):
+        _check_tensors(((name, t),), torch.bfloat16, q.device)
+        if t.shape != like.shape:
+            raise RuntimeError(f"{name} must have the shape of {name[1:]}")
+        if any(_overlap(t, other) for other in (dout, q, k, v, out, lse, *(g[1] for g in given[:i]))):
+            raise RuntimeError(f"{name} must not overlap another tensor of the call")
     grads = (torch.empty_like(q) if dq is None else dq, torch.empty_like(k) if dk is None else dk,
              torch.empty_like(v) if dv is None else dv)
     with _on(index):

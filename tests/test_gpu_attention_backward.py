@@ -239,6 +239,46 @@ def test_same_inputs_give_the_same_bits(b200, training):
         assert all(torch.equal(x, y) for x, y in zip(first, again))
 
 
+# One head over long sequences, and few rows over many keys: both plans split their work and
+# join the pieces from scratch.
+SPLIT = [(1, 1, 1, 2500, 2500, True), (1, 8, 2, 3, 9001, False), (1, 2, 1, 300, 5000, True)]
+
+
+@pytest.mark.parametrize("case", SPLIT)
+def test_split_work_on_streams_and_replayed_gives_the_same_bits(b200, training, case):
+    import torch
+
+    causal = case[5]
+    q, k, v, do = make(case, seed=17)
+
+    def layer():
+        out, lse = training.grouped_attention(q, k, v, causal)
+        return (out, lse, *training.attention_backward(do, q, k, v, out, lse, causal))
+
+    want = layer()
+    torch.cuda.synchronize()
+    graphs, kept = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept.append(layer())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):  # two replays and an eager call at once
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        again = layer()
+        torch.cuda.synchronize()
+        for got in (*kept, again):
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+        for results in kept:
+            for t in results:
+                t.fill_(float("nan"))
+        torch.cuda.synchronize()
+    del graphs
+
+
 def test_two_streams_at_once(b200, training):
     import torch
 
@@ -354,6 +394,12 @@ def test_refusals(b200, training):
 
     q, k, v, do = make((1, 4, 2, 64, 96, False), seed=15)
     out, lse = training.grouped_attention(q, k, v, False)
+    both = torch.empty((2 * k.numel(),), dtype=k.dtype, device="cuda")
+    first, second = (both[at:at + k.numel()].view(k.shape) for at in (0, k.numel() // 2))
+
+    def shifted(t):  # contiguous, but off the 16-byte grid
+        return torch.empty((t.numel() + 4,), dtype=t.dtype, device="cuda")[4:].view(t.shape)
+
     bad = [
         (lambda: training.grouped_attention(q.cpu(), k, v, False), "q must be a CUDA tensor"),
         (lambda: training.grouped_attention(q.half(), k, v, False), "q must be bf16"),
@@ -367,6 +413,11 @@ def test_refusals(b200, training):
         (lambda: training.attention_backward(do, q, k, v, out, lse[:, :2].contiguous(), False), "lse must have"),
         (lambda: training.attention_backward(do, q, k, v, out, lse.double(), False), "lse must be float32"),
         (lambda: training.attention_backward(do, q, k, v, out, lse, False, dk=torch.empty_like(q)), "dk must have"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse, False, dq=q), "dq must not overlap"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse, False, dk=v), "dk must not overlap"),
+        (lambda: training.attention_backward(do, q, k, v, out, lse, False, dk=first, dv=second), "dv must not"),
+        (lambda: training.grouped_attention(shifted(q), k, v, False), "avo_b200_attn_fwd_grouped"),
+        (lambda: training.attention_backward(do, q, shifted(k), v, out, lse, False), "avo_b200_attn_bwd"),
     ]
     for call, match in bad:
         with pytest.raises(RuntimeError, match=match):
