@@ -75,24 +75,55 @@ struct Sizes {
 };
 constexpr int kPlanSms = 148;
 
-// Pieces per item of a pass with `items` items of `longest` streamed tiles at most and `total`
-// tiles in all, whose join moves `bytes` per piece.  In microseconds: about `tile_us` for a
-// tile and three tiles' time for a unit's start and end; the join, about 4 and its bytes at
-// 4 TB/s.  One piece unless more win a tenth.
-int choose_split(double items, double longest, double total, double tile_us, double bytes) {
-  int best = 1;
-  double best_us = 0.0;
+// Pieces per item of both passes.  In microseconds: a tile takes about 1.4 (dK/dV) or 1.2 (dQ),
+// a unit's start and end five tiles more; a join about 4 and its bytes at 3 TB/s.  Units of both
+// passes that fit the chip all at once take as long as the longest.  Otherwise a dK/dV that
+// fills the chip comes first; one that does not leaves gaps, where units of dQ start early, but
+// CTAs with several of them have as many wherever they start.  One piece unless more win a
+// twentieth.  Measured on B200, one piece against the pieces chosen here (dK/dV, dQ): B1 H8
+// Hkv2 S2048 causal 92 / 42 us (4, 1), B1 H16 Hkv2 Q300 KV2048 causal 50 / 36 (2, 1), B1 H1
+// S4096 52 / 39 (2, 2), B1 H32 Hkv4 S2048 causal 217 / 117 (4, 1); but B1 H12 S1000 34 us,
+// with (2, 1) 38.
+void choose_split(Sizes& z, double kv_items, double kv_longest, double q_items, double q_longest, double total) {
+  static constexpr int kPieces[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32};
+  z.split_kv = z.split_q = 1;
   // (32 pieces keep every product of a tile count and a piece within 32 bits.)
-  if (longest * 32 > INT_MAX || items * 32 > INT_MAX) return 1;
-  for (int s = 1; s <= 32 && s <= longest; ++s) {
-    const double load = std::max(std::ceil(longest / s) + 3.0, total / kPlanSms + 3.0 * std::ceil(items * s / kPlanSms));
-    const double us = load * tile_us + (s > 1 ? 4.0 + s * bytes / 2e6 : 0.0);
-    if (s == 1 || us < (best == 1 ? 0.9 : 1.0) * best_us) {
-      best = s;
-      best_us = us;
+  if (std::max(kv_longest, q_longest) * 32 > INT_MAX || std::max(kv_items, q_items) * 32 > INT_MAX) return;
+  double best = 0.0;
+  for (const int kv : kPieces) {
+    const double kv_units = kv_items * kv;
+    if (kv > 1 && (kv > kv_longest || kv_units > 3 * kPlanSms)) break;
+    const double kv_us = 1.4 * (std::ceil(kv_longest / kv) + 5.0), kv_all = 1.4 * (total + 5.0 * kv_units);
+    for (const int q : kPieces) {
+      const double q_units = q_items * q;
+      if (q > 1 && (q > q_longest || q_units > 3 * kPlanSms)) break;
+      const double q_us = 1.2 * (std::ceil(q_longest / q) + 5.0), q_all = 1.2 * (total + 5.0 * q_units);
+      double us = std::max(kv_us, q_us);
+      if (kv_units + q_units > kPlanSms) {
+        if (kv_units >= kPlanSms) {
+          // (Units of different lengths make up for one another, equal ones do not.)
+          const bool equal = q_items * q_longest <= 1.1 * total;
+          const double q_turns = equal ? std::ceil(q_units / kPlanSms) * q_us : q_all / kPlanSms;
+          us = std::max(kv_us, kv_all / kPlanSms) + std::max(q_us, q_turns);
+        } else {
+          // (No more units of dQ then: beside dK/dV they would take up to twice as long.)
+          if (q > 1) break;
+          us = std::max({us, (kv_all + q_all) / kPlanSms, std::min(kv_all / kv_units, q_all / q_units) + q_all / q_units});
+          if (q_units > kPlanSms) us = std::max(us, kv_us + q_all / kPlanSms);
+        }
+      }
+      if (kv > 1 || q > 1) us += 4.0;
+      if (kv > 1) us += kv * 2.0 * z.part_kv / 3e6;
+      if (q > 1) us += q * 1.0 * z.part_q / 3e6;
+      if (kv == 1 && q == 1) {
+        best = 0.95 * us;
+      } else if (us < best) {
+        best = us;
+        z.split_kv = kv;
+        z.split_q = q;
+      }
     }
   }
-  return best;
 }
 
 Sizes sizes_of(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal) {
@@ -122,9 +153,7 @@ Sizes sizes_of(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int ca
     pairs = std::min(pairs, seen / (kTile * kTile) + 0.5 * tiles_of(std::min(seq_q, seq_kv)));
   }
   const double kv_items = static_cast<double>(z.kv_heads) * z.nkv, q_items = static_cast<double>(z.q_heads) * z.nq;
-  const double total = pairs * z.q_heads;
-  z.split_kv = choose_split(kv_items, static_cast<double>(z.group) * z.nq, total, 1.35, 2.0 * z.part_kv);
-  z.split_q = choose_split(q_items, z.nkv, total, 1.0, static_cast<double>(z.part_q));
+  choose_split(z, kv_items, static_cast<double>(z.group) * z.nq, q_items, z.nkv, pairs * z.q_heads);
   return z;
 }
 
@@ -138,8 +167,11 @@ void set_items(bwd::BwdParams& p, int heads, int tiles, int split) {
   p.item_magic = ~0ull / p.item_div + 1;
 }
 
+constexpr size_t kClaimBytes = 2 * bwd::kMaxClaims * sizeof(uint32_t);
+
+// Claims and row statistics.
 size_t stats_bytes(const Sizes& z) {
-  return round256(static_cast<size_t>(z.q_heads) * z.nq * bwd::kStatBytes);
+  return round256(static_cast<size_t>(z.q_heads) * z.nq * bwd::kStatBytes + kClaimBytes);
 }
 
 size_t scratch_bytes(const Sizes& z) {
@@ -202,7 +234,9 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   if ((rc = host::encode(&tv, v, z.seq_kv, z.kv_heads)) != AVO_B200_OK) return rc;
 
   bwd::BwdParams p{};
-  p.stats = static_cast<const float*>(workspace);
+  uint32_t* const claims = static_cast<uint32_t*>(workspace);
+  float* const stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + kClaimBytes);
+  p.stats = stats;
   p.status = status_dev;
   p.watchdog_ns = host::watchdog_limit();
   p.seq_q = z.seq_q;
@@ -223,34 +257,36 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
 
   const long long kv_units = static_cast<long long>(z.kv_heads) * z.nkv * z.split_kv;
   const long long q_units = static_cast<long long>(z.q_heads) * z.nq * z.split_q;
-  // Both passes at once where the dK/dV grid leaves multiprocessors idle from the start.
-  // Measured on B200, at once against one after the other: B1 H4 S512 14.1 / 22.9 us, B1 H16
-  // Hkv2 Q777 KV5003 137 / 144 us; but B1 H16 S4096 493 / 417 us: both passes slow down while
-  // they share the chip.
-  p.overlap = kv_units < sms ? 1 : 0;
+  // With a unit for every multiprocessor, CTAs take them by place (see the kernel).  Not with
+  // fewer: the two passes then share the chip from the start, and CTAs without a unit would
+  // leave their places to later ones on the same multiprocessor (measured on B200, B1 H8 S2048,
+  // 128 units a pass: 54 us, with places and idle CTAs 110).
+  const bool by_place = kv_units >= sms && sms <= bwd::kMaxClaims;
+  const unsigned kv_grid = static_cast<unsigned>(kv_units > sms ? sms : kv_units);
+  const unsigned q_grid = static_cast<unsigned>(q_units > sms ? sms : q_units);
 
   const long long rows = static_cast<long long>(z.q_heads) * p.nq * kTile;
   const long long blocks = rows / 16;
   if (blocks > INT_MAX) return AVO_B200_EINVAL;
   if (!host::launch_early(bwd::stats_kernel, static_cast<unsigned>(blocks), 256u, 0, st,
                           static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse,
-                          static_cast<float*>(workspace), rows, z.seq_q, p.nq))
+                          stats, rows, z.seq_q, p.nq, claims))
     return AVO_B200_ELAUNCH;
   set_items(p, z.kv_heads, z.nkv, z.split_kv);
+  p.claims = by_place ? claims : nullptr;
   p.g1 = dk;
   p.g2 = dv;
   p.part1 = part_dk;
   p.part2 = part_dv;
-  if (!host::launch_early(bwd::attn_bwd_kernel<false>, static_cast<unsigned>(kv_units < sms ? kv_units : sms),
-                          bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tk, tv, tq, tdo, p))
+  if (!host::launch_early(bwd::attn_bwd_kernel<false>, kv_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tk, tv, tq, tdo, p))
     return AVO_B200_ELAUNCH;
   set_items(p, z.q_heads, z.nq, z.split_q);
+  p.claims = by_place && q_units >= sms ? claims + bwd::kMaxClaims : nullptr;
   p.g1 = dq;
   p.g2 = nullptr;
   p.part1 = part_dq;
   p.x1 = q;
-  if (!host::launch_early(bwd::attn_bwd_kernel<true>, static_cast<unsigned>(q_units < sms ? q_units : sms),
-                          bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
+  if (!host::launch_early(bwd::attn_bwd_kernel<true>, q_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
     return AVO_B200_ELAUNCH;
   if (z.split_kv > 1 || z.split_q > 1) {
     bwd::JoinParams j{};

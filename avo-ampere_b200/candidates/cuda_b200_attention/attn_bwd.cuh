@@ -35,7 +35,7 @@
 // K slot), so S_{n+1} and dP_{n+1} start as soon as S_n and dP_n are in registers.
 //
 // Sums are fp32 in TMEM; P and dS are rounded once to bf16 (the type of the tensor cores'
-// operands: half a step, 2^-9 of each value), the gradients once at the end.
+// operands: at most half a step, 2^-8 of each value), the gradients once at the end.
 //
 // Roles (768 threads): warps 0-15 softmax (four warpgroups, 32 of a tile's 128 columns each),
 // warps 16-19 the epilogue (an item's accumulators to memory, and Q of the next item to TMEM,
@@ -151,8 +151,11 @@ enum : int {
 };
 constexpr int kSmTmem = kSmBars + B_COUNT * 8;
 constexpr int kSmAbort = kSmTmem + 4;
-constexpr int kBwdSmemBytes = (kSmAbort + 4 + 15) / 16 * 16;
+constexpr int kSmSlot = kSmAbort + 4;  // this CTA's place in the order of items
+constexpr int kBwdSmemBytes = (kSmSlot + 4 + 15) / 16 * 16;
 static_assert(kBwdSmemBytes <= 227 * 1024, "shared memory budget");
+
+constexpr int kMaxClaims = 256;  // multiprocessors, at most, whose CTAs claim a place
 
 // TMEM columns: T1 | T2 | accumulator 1 | accumulator 2 (dK/dV) or dS and Q (dQ).
 constexpr uint32_t kColT1 = 0, kColT2 = 128, kColAcc1 = 256, kColAcc2 = 384;
@@ -172,7 +175,7 @@ struct BwdParams {
   int causal;
   int offset;              // causal: key j is visible to query i iff j <= i + offset
   float scale, scale_log2;
-  int overlap;             // the two passes may run at the same time
+  uint32_t* claims;        // null (one item per CTA at most), or gridDim.x zeros: places taken
   int test_skip_load;
   // An item is a stationary tile; with split > 1 it is cut into that many pieces along the
   // streamed tiles, each a unit of its own whose sums go to part1 / part2 in fp32
@@ -203,7 +206,8 @@ struct Items {
   int n;           // streamed tiles of this unit (dK/dV: over the whole group of heads)
   int skip;        // of the item's tiles, those of earlier pieces
   int piece;
-  __device__ explicit Items(const BwdParams& params) : p(params) {}
+  const volatile uint32_t* slot;
+  __device__ Items(const BwdParams& params, const volatile uint32_t* place) : p(params), slot(place) {}
   // The next item that has tiles.
   __device__ bool next_busy() {
     do {
@@ -212,7 +216,7 @@ struct Items {
     return true;
   }
   __device__ bool next() {
-    const uint32_t grid = gridDim.x, cta = blockIdx.x;
+    const uint32_t grid = gridDim.x, cta = *slot;
     while (true) {
       const unsigned long long base = static_cast<unsigned long long>(r) * grid;
       if (base >= p.item_count) return false;
@@ -261,7 +265,7 @@ struct Tiles {
   int left = 0;   // tiles of the item still to come
   int t, y_head;  // current streamed tile and its head
   bool first, last;
-  __device__ explicit Tiles(const BwdParams& params) : items(params) {}
+  __device__ Tiles(const BwdParams& params, const volatile uint32_t* place) : items(params, place) {}
   __device__ bool next() {
     first = false;
     if (left == 0) {
@@ -362,6 +366,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int lane = threadIdx.x & 31;
   auto bar = [&](int idx) -> uint32_t { return sbase + kSmBars + idx * 8; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmAbort);
+  volatile uint32_t* slot = reinterpret_cast<volatile uint32_t*>(smem + kSmSlot);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmTmem);
   const Watch watch{abort_flag, p.status, p.watchdog_ns};
 
@@ -373,6 +378,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < B_COUNT; ++b) mbar_init(bar(b), 1);
     *abort_flag = 0;
+    *slot = blockIdx.x;
     fence_mbarrier_init();
   }
   if (warp == kProducerWarp && lane == 0) {
@@ -391,10 +397,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // The dK/dV launch follows stats_kernel and waits for it here.  The dQ launch follows the
   // dK/dV launch, reads nothing that it writes, and can only start once all CTAs of that
-  // launch have passed this wait.  With p.overlap it runs at the same time, on the
-  // multiprocessors that launch leaves free, and waits for it at its own end.
-  if (!kDq || !p.overlap) grid_dependency_wait();
-  if (!kDq) grid_launch_dependents();
+  // launch have passed this wait; it runs on the multiprocessors that launch leaves free, or
+  // is done with, and its last CTA waits for it at the end.
+  if (!kDq) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
+  // CTAs with several items take their place in the order of items by multiprocessor (the next
+  // free one, should two CTAs ask for the same), and dQ counts from the other end.  Then a
+  // multiprocessor that has one item more of dK/dV has the fewest of dQ, and the two of a pair
+  // (a TPC) change from one pass to the other at the same time: while they run different
+  // kernels, both take up to twice as long (the pair seems to share its instruction cache).
+  // Measured on B200, B1 H16 S4096: both passes one after
+  // the other 391 to 413 us, at once without such places 411 to 447, with them 335 to 381.
+  if (p.claims != nullptr) {
+    if (threadIdx.x == 0) {
+      const uint32_t grid = gridDim.x;
+      uint32_t s = sm_id() % grid;
+      for (uint32_t i = 0; i < grid && atomicExch(p.claims + s, 1u) != 0u; ++i) s = s + 1 == grid ? 0 : s + 1;
+      *slot = kDq ? grid - 1 - s : s;
+    }
+    __syncthreads();
+  }
 
   if (warp < kEpiWarp) {
     regs_increase<kBwdRegsSoftmax>();
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     uint32_t n = 0;
     float neg_lse = 0.f, neg_delta = 0.f;
-    Tiles<kDq> it(p);
+    Tiles<kDq> it(p, slot);
     // The barrier rounds of a tile from round `from` on, blocking: after an abort a warp
     // keeps its place in the issuer's schedule with these.
     auto keep_rounds = [&](int from) {
@@ -423,7 +447,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       named_bar_sync(bar_tile(kRoundDs, n), kDsThreads<kDq>);
     };
     // dQ: the statistics of this row in the item after the current one, loaded an item ahead.
-    Items<kDq> ahead(p);
+    Items<kDq> ahead(p, slot);
     float next_lse = 0.f, next_delta = 0.f;
     auto load_stats = [&]() {
       if (!ahead.next_busy()) return;
@@ -596,7 +620,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     uint32_t done = 0;   // items with tiles so far
     // dQ: this thread's row of Q of the next item with tiles, its first half loaded an item
     // ahead, the second when it is stored.
-    Items<kDq> ahead(p);
+    Items<kDq> ahead(p, slot);
     uint32_t xq[32];
     bool have_x = false;
     auto load_half = [&](int half) {
@@ -636,7 +660,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       load_x();
       if (have_x) store_x();
     }
-    Items<kDq> it(p);
+    Items<kDq> it(p, slot);
     while (ok && it.next()) {
       if (kDq && it.n > 0) {
         load_x();
@@ -708,7 +732,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!kDq && acc_seen++ >= acc_signals) named_bar_sync(bar_acc2(i), kEpiThreads);
         if (acc_seen++ >= acc_signals) named_bar_sync(bar_acc1(i), kEpiThreads);
       };
-      Items<kDq> all(p), after(p);
+      Items<kDq> all(p, slot), after(p, slot);
       bool more = after.next_busy();
       if (kDq && more) x_round();
       for (; all.next_busy(); ++item) {
@@ -745,13 +769,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // The stationary tiles of the next item, and its first streamed ones, are brought to L2
       // while this item runs: their loads start only when its last tiles are done with the
       // buffers.
-      Items<kDq> ahead(p);
+      Items<kDq> ahead(p, slot);
       ahead.next_busy();
       auto prefetch = [&](const CUtensorMap* tm, int r0, int head) {
         tma_prefetch_3d(tm, 0, r0, head);
         tma_prefetch_3d(tm, 64, r0, head);
       };
-      Tiles<kDq> it(p);
+      Tiles<kDq> it(p, slot);
       while (it.next()) {
         if (it.first && ahead.next_busy()) {
           const int y_head = kDq ? ahead.head / p.group : ahead.head * p.group;
@@ -825,7 +849,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       named_bar_sync(id, threads);
       tc_fence_after();
     };
-    Tiles<kDq> it(p);
+    Tiles<kDq> it(p, slot);
     uint32_t items = 0;
     auto issue_t1 = [&](int slot, int parity) {
       if constexpr (kDq)
@@ -906,7 +930,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // for T2); then its rounds on the barriers whose release lets the issuer use them.  After
     // an abort the waits return at once and only the rounds are kept.
     int n1 = 0, n2 = 0, x1 = 0, x2 = 0;
-    Tiles<kDq> a(p), c(p);  // tiles whose T1 / T2 operands are next
+    Tiles<kDq> a(p, slot), c(p, slot);  // tiles whose T1 / T2 operands are next
     auto t1_loaded = [&]() {
       if (!a.next()) return;
       if (lane == 0) {
@@ -929,7 +953,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       named_bar_sync(id, threads);
     };
-    Tiles<kDq> it(p);
+    Tiles<kDq> it(p, slot);
     bool have = it.next();
     if (have) {
       t1_loaded();
@@ -953,8 +977,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-  // The dQ launch is complete only when the dK/dV launch is (see above).
-  if (kDq && p.overlap) grid_dependency_wait();
+  // The dQ launch is complete only when the dK/dV launch is (see above).  One CTA waits for
+  // that; the others make room.
+  if (kDq && blockIdx.x == gridDim.x - 1) grid_dependency_wait();
 }
 
 // The sums of split units: out = bf16(factor * (part[0] + part[1] + ...)), in this order, for
@@ -992,9 +1017,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinP
 // (LSE = -inf) get -inf, so their probabilities are exactly 0.
 __global__ void __launch_bounds__(256)
     stats_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ out, const float* __restrict__ lse,
-                 float* __restrict__ stats, long long rows_padded, int seq_q, int nq) {
+                 float* __restrict__ stats, long long rows_padded, int seq_q, int nq, uint32_t* claims) {
   grid_dependency_wait();
   grid_launch_dependents();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < 2 * kMaxClaims; i += blockDim.x) claims[i] = 0u;
   const long long g = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
   const int l = threadIdx.x & 15;
   if (g >= rows_padded) return;  // whole warps: rows_padded is a multiple of 128
