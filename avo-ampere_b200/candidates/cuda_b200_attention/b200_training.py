@@ -131,7 +131,7 @@ def _forward(q, k, v, causal: bool, scale: float):
     torch = _torch()
     batch, heads, kv_heads, seq_q, seq_kv = _attention_shape(q, k, v)
     out = torch.empty_like(q)
-    lse = torch.empty((batch, heads, seq_q), dtype=torch.float32, device=q.device)
+    lse = q.new_empty((batch, heads, seq_q), dtype=torch.float32)
     if out.numel() == 0:
         return out, lse
     if seq_kv == 0:
@@ -140,7 +140,7 @@ def _forward(q, k, v, causal: bool, scale: float):
     index = q.get_device()
     with _on(index):
         size = _forward_scratch_bytes(index)
-        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(size, dtype=torch.uint8)
         code = b.call_entry(
             0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,
             seq_kv, HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_address(index),
@@ -256,7 +256,7 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
              torch.empty_like(v) if dv is None else dv)
     with _on(index):
         size = _backward_scratch_bytes(batch, heads, kv_heads, seq_q, seq_kv, bool(causal))
-        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(size, dtype=torch.uint8)
         code = b.call_entry(
             1, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), batch, heads, kv_heads, seq_q, seq_kv,
@@ -352,8 +352,8 @@ def _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, se
     torch = _torch()
     batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
                                         interleaved)
-    q = torch.empty((batch, heads, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
-    k = torch.empty((batch, kv_heads, seq, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((batch, heads, seq, HEAD_DIM))
+    k = qkv.new_empty((batch, kv_heads, seq, HEAD_DIM))
     v = torch.empty_like(k)
     if qkv.numel() == 0:
         return q, k, v
@@ -386,15 +386,15 @@ def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight
                                         interleaved)
     if tuple(dq.shape) != (batch, heads, seq, HEAD_DIM) or tuple(dk.shape) != (batch, kv_heads, seq, HEAD_DIM):
         raise RuntimeError("dq, dk and dv must match qkv's batch and sequence")
-    dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+    dqkv = qkv.new_empty(qkv.shape)
     b.load_library()
     index = qkv.get_device()
     with _on(index):
         weights, scratch, size = (None, None), None, 0
         if q_weight is not None:
-            weights = tuple(torch.empty((2, HEAD_DIM), dtype=torch.float32, device=qkv.device).unbind())
+            weights = cos.new_empty((2, HEAD_DIM)).unbind()
             size = _rope_scratch_bytes(index)
-            scratch = torch.empty(size, dtype=torch.uint8, device=qkv.device)
+            scratch = qkv.new_empty(size, dtype=torch.uint8)
         code = b.call_entry(
             3, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), *_qkv_strides(qkv), dqkv.data_ptr(),
             None if q_weight is None else weights[0].data_ptr(), None if q_weight is None else weights[1].data_ptr(),
