@@ -16,6 +16,13 @@ using bwd::kTile;
 
 int tiles_of(int rows) { return rows / kTile + (rows % kTile != 0); }
 
+template <bool kDq>
+auto kernel_of(bwd::Order order) {
+  return order == bwd::kPairs   ? bwd::attn_bwd_kernel<kDq, bwd::kPairs>
+         : order == bwd::kEqual ? bwd::attn_bwd_kernel<kDq, bwd::kEqual>
+                                : bwd::attn_bwd_kernel<kDq, bwd::kAny>;
+}
+
 // The kernels' shared-memory limit and register allocation, once per device.
 int prepare_bwd(int* sm_count) {
   const int rc = host::device(sm_count);
@@ -27,8 +34,12 @@ int prepare_bwd(int* sm_count) {
     return AVO_B200_ENODEV;
   }
   if (dev < 64 && ready[dev].load(std::memory_order_acquire) == 1) return AVO_B200_OK;
-  const void* kernels[] = {reinterpret_cast<const void*>(bwd::attn_bwd_kernel<false>),
-                           reinterpret_cast<const void*>(bwd::attn_bwd_kernel<true>)};
+  const void* kernels[] = {reinterpret_cast<const void*>(kernel_of<false>(bwd::kAny)),
+                           reinterpret_cast<const void*>(kernel_of<true>(bwd::kAny)),
+                           reinterpret_cast<const void*>(kernel_of<false>(bwd::kEqual)),
+                           reinterpret_cast<const void*>(kernel_of<true>(bwd::kEqual)),
+                           reinterpret_cast<const void*>(kernel_of<false>(bwd::kPairs)),
+                           reinterpret_cast<const void*>(kernel_of<true>(bwd::kPairs))};
   for (const void* k : kernels) {
     cudaFuncAttributes attr{};
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd::kBwdSmemBytes) != cudaSuccess ||
@@ -159,11 +170,32 @@ Sizes sizes_of(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int ca
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
-void set_items(bwd::BwdParams& p, int heads, int tiles, int split) {
+// Causal items are taken in pairs where whole pairs leave less than a twentieth of the
+// multiprocessors' time idle.  Longest first balances any number of items, but has all heads in
+// flight at once: where they do not fit L2 they are read from memory again and again, and that
+// takes power from the multiprocessors' clock (measured on B200, longest first against pairs,
+// back to back at the power limit: B8 H16 S2048 590 us at 1.17 GHz / 525 at 1.45, B2 H16 S8192
+// 1690 / 1590, B16 H16 S1024 383 / 350; but B1 H16 S4096, 1.7 pairs to a multiprocessor,
+// 220 / 240).
+bwd::Order order_of(const Sizes& z, int sms) {
+  if (z.split_kv > 1 || z.split_q > 1) return bwd::kAny;
+  if (!z.causal) return bwd::kEqual;
+  if (z.offset != 0) return bwd::kAny;
+  const long long kv = z.kv_heads * ((z.nkv + 1LL) / 2), q = z.q_heads * ((z.nq + 1LL) / 2);
+  const double kv_us = 1.4 * (z.group * (z.nq + 1.0) + 10.0), q_us = 1.2 * (z.nkv + 1.0 + 10.0);
+  // Multiprocessors with one pair more of dK/dV are the last to have one more of dQ.
+  const long long kv_more = kv % sms, q_more = q % sms;
+  double most = kv_more + q_more > sms ? kv_us + q_us : std::max(kv_more > 0 ? kv_us : 0.0, q_more > 0 ? q_us : 0.0);
+  most += kv / sms * kv_us + q / sms * q_us;
+  return most * 0.95 * sms < kv * kv_us + q * q_us ? bwd::kPairs : bwd::kAny;
+}
+
+void set_items(bwd::BwdParams& p, int heads, int tiles, int split, bwd::Order order) {
   p.split = static_cast<uint32_t>(split);
   p.split_magic = ~0ull / p.split + 1;  // unused for 1
-  p.item_count = static_cast<uint32_t>(heads) * static_cast<uint32_t>(tiles) * p.split;
-  p.item_div = static_cast<uint32_t>(p.causal ? heads : tiles);
+  const int rows = order == bwd::kPairs ? (tiles + 1) / 2 : tiles;
+  p.item_count = static_cast<uint32_t>(heads) * static_cast<uint32_t>(rows) * p.split;
+  p.item_div = static_cast<uint32_t>(p.causal && order == bwd::kAny ? heads : rows);
   p.item_magic = ~0ull / p.item_div + 1;
 }
 
@@ -255,6 +287,7 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   float* const part_dv = part_dk + (z.split_kv > 1 ? z.split_kv * z.part_kv / sizeof(float) : 0);
   float* const part_dq = part_dv + (z.split_kv > 1 ? z.split_kv * z.part_kv / sizeof(float) : 0);
 
+  const bwd::Order order = order_of(z, sms);
   const long long kv_units = static_cast<long long>(z.kv_heads) * z.nkv * z.split_kv;
   const long long q_units = static_cast<long long>(z.q_heads) * z.nq * z.split_q;
   // With a unit for every multiprocessor, CTAs take them by place (see the kernel).  Not with
@@ -272,21 +305,21 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
                           static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse,
                           stats, rows, z.seq_q, p.nq, claims))
     return AVO_B200_ELAUNCH;
-  set_items(p, z.kv_heads, z.nkv, z.split_kv);
+  set_items(p, z.kv_heads, z.nkv, z.split_kv, order);
   p.claims = by_place ? claims : nullptr;
   p.g1 = dk;
   p.g2 = dv;
   p.part1 = part_dk;
   p.part2 = part_dv;
-  if (!host::launch_early(bwd::attn_bwd_kernel<false>, kv_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tk, tv, tq, tdo, p))
+  if (!host::launch_early(kernel_of<false>(order), kv_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tk, tv, tq, tdo, p))
     return AVO_B200_ELAUNCH;
-  set_items(p, z.q_heads, z.nq, z.split_q);
+  set_items(p, z.q_heads, z.nq, z.split_q, order);
   p.claims = by_place && q_units >= sms ? claims + bwd::kMaxClaims : nullptr;
   p.g1 = dq;
   p.g2 = nullptr;
   p.part1 = part_dq;
   p.x1 = q;
-  if (!host::launch_early(bwd::attn_bwd_kernel<true>, q_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
+  if (!host::launch_early(kernel_of<true>(order), q_grid, bwd::kBwdThreads, bwd::kBwdSmemBytes, st, tq, tdo, tk, tv, p))
     return AVO_B200_ELAUNCH;
   if (z.split_kv > 1 || z.split_q > 1) {
     bwd::JoinParams j{};

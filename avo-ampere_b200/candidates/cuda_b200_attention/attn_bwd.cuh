@@ -75,7 +75,7 @@ static_assert(kSoftmaxThreads * kBwdRegsSoftmax + 128 * kBwdRegsEpi + 128 * kBwd
 // of the item's tiles has a watchdog of its own, so their sum bounds this wait.
 __device__ __forceinline__ bool wait_item(uint32_t bar, uint32_t parity, int tiles, const Watch& w, int lane) {
   bool ok = true;
-  if (lane == 0) {
+  if (lane == 0 && !mbar_try_wait(bar, parity)) {
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait_sleep(bar, parity, 20000)) {
       ok = !*w.abort;
@@ -184,8 +184,8 @@ struct BwdParams {
   unsigned long long split_magic;
   float* part1;
   float* part2;
-  uint32_t item_count;     // units of this launch
-  uint32_t item_div;       // what an item's number is divided by: heads (causal) or tiles
+  uint32_t item_count;     // units, or pairs, of this launch
+  uint32_t item_div;       // what an item's number is divided by: heads (causal), tiles or pairs of them
   unsigned long long item_magic;
 };
 
@@ -195,9 +195,20 @@ __device__ __forceinline__ uint32_t div_by(uint32_t w, uint32_t div, unsigned lo
   return div == 1 ? w : static_cast<uint32_t>(__umul64hi(w, magic));
 }
 
-// One CTA's units in order (a stationary tile of one head, or a piece of its work): waves over
-// the grid in alternating directions, causal items longest first.
-template <bool kDq>
+// The order of the items, and what the kernel is compiled for.  The two cases with the most work
+// are simpler than the general one, and the softmax warps, short of registers, gain by that
+// (measured on B200, compiled for all cases / for its own: B4 H16 S4096 1547 / 1528 us; causal
+// B8 H16 S2048, in pairs in either, 545 / 520).
+//   kAny    waves over the grid in alternating directions.  Causal items are of different
+//           lengths: longest first, the same tile of all heads before the next tile.
+//   kEqual  (no mask, whole items) the same, heads one after the other.
+//   kPairs  (causal, equal lengths, whole items) heads one after the other, and each CTA takes
+//           the first and the last tile of a head, or the second and the last but one, and so
+//           on, which together are as long as any other pair.
+enum Order : int { kAny, kEqual, kPairs };
+
+// One CTA's units in order (a stationary tile of one head, or a piece of its work).
+template <bool kDq, Order kOrder>
 struct Items {
   const BwdParams& p;
   uint32_t r = 0;
@@ -218,23 +229,47 @@ struct Items {
   __device__ bool next() {
     const uint32_t grid = gridDim.x, cta = *slot;
     while (true) {
-      const unsigned long long base = static_cast<unsigned long long>(r) * grid;
-      if (base >= p.item_count) return false;
-      const uint32_t unit = static_cast<uint32_t>(base) + ((r & 1) ? grid - 1 - cta : cta);
-      ++r;
-      if (unit >= p.item_count) continue;
-      const uint32_t w = div_by(unit, p.split, p.split_magic);
-      piece = static_cast<int>(unit - w * p.split);
-      const uint32_t quotient = div_by(w, p.item_div, p.item_magic);
-      const int rest = static_cast<int>(w - quotient * p.item_div);
-      if (p.causal) {
-        head = rest;
-        tile = kDq ? p.nq - 1 - static_cast<int>(quotient) : static_cast<int>(quotient);
-      } else {
+      if constexpr (kOrder == kPairs) {
+        const unsigned long long at = static_cast<unsigned long long>(r >> 1) * grid + cta;
+        if (at >= p.item_count) return false;
+        const uint32_t quotient = div_by(static_cast<uint32_t>(at), p.item_div, p.item_magic);
         head = static_cast<int>(quotient);
-        tile = rest;
+        tile = static_cast<int>(static_cast<uint32_t>(at) - quotient * p.item_div);
+        if (r++ & 1) {
+          const int partner = (kDq ? p.nq : p.nkv) - 1 - tile;
+          if (partner == tile) continue;  // the middle tile
+          tile = partner;
+        }
+        piece = 0;
+      } else {
+        const unsigned long long base = static_cast<unsigned long long>(r) * grid;
+        if (base >= p.item_count) return false;
+        const uint32_t unit = static_cast<uint32_t>(base) + ((r & 1) ? grid - 1 - cta : cta);
+        ++r;
+        if (unit >= p.item_count) continue;
+        const uint32_t w = kOrder == kEqual ? unit : div_by(unit, p.split, p.split_magic);
+        piece = kOrder == kEqual ? 0 : static_cast<int>(unit - w * p.split);
+        const uint32_t quotient = div_by(w, p.item_div, p.item_magic);
+        const int rest = static_cast<int>(w - quotient * p.item_div);
+        if (kOrder == kAny && p.causal) {
+          head = rest;
+          tile = kDq ? p.nq - 1 - static_cast<int>(quotient) : static_cast<int>(quotient);
+        } else {
+          head = static_cast<int>(quotient);
+          tile = rest;
+        }
       }
       t0 = 0;
+      skip = 0;
+      if constexpr (kOrder == kPairs) {
+        if (!kDq) t0 = tile;
+        n = kDq ? tile + 1 : (p.nq - tile) * p.group;
+        return true;
+      }
+      if constexpr (kOrder == kEqual) {
+        n = kDq ? p.nkv : p.nq * p.group;
+        return true;
+      }
       if (kDq) {
         n = p.nkv;
         if (p.causal) {
@@ -247,7 +282,6 @@ struct Items {
         if (p.causal && tile * kTile - p.offset >= p.seq_q) t0 = p.nq;
         n = (p.nq - t0) * p.group;
       }
-      skip = 0;
       if (p.split > 1) {
         const uint32_t all = static_cast<uint32_t>(n), pieces = p.split, at = static_cast<uint32_t>(piece);
         skip = static_cast<int>(div_by(all * at, pieces, p.split_magic));
@@ -259,9 +293,9 @@ struct Items {
 };
 
 // The tiles of a CTA's items as one sequence (items without tiles are skipped).
-template <bool kDq>
+template <bool kDq, Order kOrder>
 struct Tiles {
-  Items<kDq> items;
+  Items<kDq, kOrder> items;
   int left = 0;   // tiles of the item still to come
   int t, y_head;  // current streamed tile and its head
   bool first, last;
@@ -274,7 +308,7 @@ struct Tiles {
       first = true;
       t = items.t0 + items.skip;
       y_head = kDq ? items.head / items.p.group : items.head * items.p.group;
-      if (!kDq && items.skip > 0) {
+      if (!kDq && kOrder == kAny && items.skip > 0) {
         const int per_head = items.p.nq - items.t0;
         const int heads = items.skip / per_head;
         y_head += heads;
@@ -353,12 +387,14 @@ __device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
   return pack_bf16x2(a, b);
 }
 
-template <bool kDq>
+template <bool kDq, Order kOrder>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__ CUtensorMap tm_x2,
                     const __grid_constant__ CUtensorMap tm_y1, const __grid_constant__ CUtensorMap tm_y2,
                     const __grid_constant__ BwdParams p) {
   using Sm = Smem<kDq>;
+  using Items = bwd::Items<kDq, kOrder>;
+  using Tiles = bwd::Tiles<kDq, kOrder>;
   constexpr int kY1 = Sm::kY1;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_addr(smem);
@@ -430,9 +466,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int row = threadIdx.x & 127;
     const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 16;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    const bool causal = kOrder == kPairs || (kOrder == kAny && p.causal);
+    const int offset = kOrder == kPairs ? 0 : p.offset;
     uint32_t n = 0;
     float neg_lse = 0.f, neg_delta = 0.f;
-    Tiles<kDq> it(p, slot);
+    Tiles it(p, slot);
     // The barrier rounds of a tile from round `from` on, blocking: after an abort a warp
     // keeps its place in the issuer's schedule with these.
     auto keep_rounds = [&](int from) {
@@ -447,7 +485,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       named_bar_sync(bar_tile(kRoundDs, n), kDsThreads<kDq>);
     };
     // dQ: the statistics of this row in the item after the current one, loaded an item ahead.
-    Items<kDq> ahead(p, slot);
+    Items ahead(p, slot);
     float next_lse = 0.f, next_delta = 0.f;
     auto load_stats = [&]() {
       if (!ahead.next_busy()) return;
@@ -482,8 +520,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // 7 to 20 %: the one splits the block that the scheduler interleaves, the other spills.)
       if (masked) {
         const int r = it.items.tile * kTile + row, c0 = it.t * kTile;
-        const int lo = kDq ? 0 : r - p.offset - c0;
-        const int hi = kDq ? (p.causal ? min(p.seq_kv, r + p.offset + 1) : p.seq_kv) - c0 : kTile;
+        const int lo = kDq ? 0 : r - offset - c0;
+        const int hi = kDq ? (causal ? min(p.seq_kv, r + offset + 1) : p.seq_kv) - c0 : kTile;
 #pragma unroll 1
         for (int c = 0; c < kTile; c += 64) {
           uint32_t s[16];
@@ -595,12 +633,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         full_lo = 0;
         full_hi = INT_MAX;
         if (kDq) {
-          full_hi = p.causal ? max(0, min(p.seq_kv, r0 + p.offset + 1)) / kTile : p.seq_kv / kTile;
+          full_hi = causal ? max(0, min(p.seq_kv, r0 + offset + 1)) / kTile : p.seq_kv / kTile;
           neg_lse = next_lse;
           neg_delta = next_delta;
           load_stats();
-        } else if (p.causal) {
-          full_lo = (max(0, r0 + 31 - p.offset) + kTile - 1) / kTile;
+        } else if (causal) {
+          full_lo = (max(0, r0 + 31 - offset) + kTile - 1) / kTile;
         }
       }
       failed = one_tile(it.t < full_lo || it.t >= full_hi);
@@ -620,7 +658,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     uint32_t done = 0;   // items with tiles so far
     // dQ: this thread's row of Q of the next item with tiles, its first half loaded an item
     // ahead, the second when it is stored.
-    Items<kDq> ahead(p, slot);
+    Items ahead(p, slot);
     uint32_t xq[32];
     bool have_x = false;
     auto load_half = [&](int half) {
@@ -660,7 +698,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       load_x();
       if (have_x) store_x();
     }
-    Items<kDq> it(p, slot);
+    Items it(p, slot);
     while (ok && it.next()) {
       if (kDq && it.n > 0) {
         load_x();
@@ -689,31 +727,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (!ok) break;
           tc_fence_after();
         }
+        // The next 16 columns are on their way while these are stored.
+        uint32_t o[2][16];
+        if (it.n > 0) {
+          tmem_ld16(acc, o[0]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[0][e] = o[1][e] = 0u;
+        }
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          uint32_t o[16];
+          uint32_t* const x = o[c & 1];
           if (it.n > 0) {
-            tmem_ld16(acc + c * 16, o);
-            tmem_wait_ld16(o);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0u;
+            tmem_wait_ld16(o[c & 1]);
+            if (c < 7) {
+              tmem_ld16(acc + (c + 1) * 16, o[(c + 1) & 1]);
+            } else {
+              // Read out: the next item may overwrite it.
+              tc_fence_before();
+              __syncwarp();
+              named_bar_arrive(a == 1 ? bar_acc1(done) : bar_acc2(done), kEpiThreads);
+              ++acc_signals;
+            }
           }
-          if (c == 7 && it.n > 0) {
-            // Read out: the next item may overwrite it.
-            tc_fence_before();
-            __syncwarp();
-            named_bar_arrive(a == 1 ? bar_acc1(done) : bar_acc2(done), kEpiThreads);
-            ++acc_signals;
-          }
-          if (write && p.split > 1) {
+          if (kOrder == kAny && write && p.split > 1) {
 #pragma unroll
             for (int e = 0; e < 16; e += 8)
-              st_global_v8(part + c * 16 + e, o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+              st_global_v8(part + c * 16 + e, x[e], x[e + 1], x[e + 2], x[e + 3], x[e + 4], x[e + 5], x[e + 6], x[e + 7]);
           } else if (write) {
             uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(u2f(o[2 * e]) * f, u2f(o[2 * e + 1]) * f);
+            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(u2f(x[2 * e]) * f, u2f(x[2 * e + 1]) * f);
             st_global_v8(dst + c * 16, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
           }
         }
@@ -732,7 +776,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!kDq && acc_seen++ >= acc_signals) named_bar_sync(bar_acc2(i), kEpiThreads);
         if (acc_seen++ >= acc_signals) named_bar_sync(bar_acc1(i), kEpiThreads);
       };
-      Items<kDq> all(p, slot), after(p, slot);
+      Items all(p, slot), after(p, slot);
       bool more = after.next_busy();
       if (kDq && more) x_round();
       for (; all.next_busy(); ++item) {
@@ -767,23 +811,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       auto reuse = [&](int commit, int u) { return reuse_after(commit + (u & 1), (u >> 1) & 1); };
       int n = 0, n2 = 0, nx1 = 0, nx2 = 0, nst = 0, skipped = -1;
       // The stationary tiles of the next item, and its first streamed ones, are brought to L2
-      // while this item runs: their loads start only when its last tiles are done with the
-      // buffers.
-      Items<kDq> ahead(p, slot);
+      // while this item runs, once its own first loads are on their way: their loads start only
+      // when its last tiles are done with the buffers.
+      Items ahead(p, slot);
       ahead.next_busy();
       auto prefetch = [&](const CUtensorMap* tm, int r0, int head) {
         tma_prefetch_3d(tm, 0, r0, head);
         tma_prefetch_3d(tm, 64, r0, head);
       };
-      Tiles<kDq> it(p, slot);
+      Tiles it(p, slot);
       while (it.next()) {
-        if (it.first && ahead.next_busy()) {
-          const int y_head = kDq ? ahead.head / p.group : ahead.head * p.group;
-          if (!kDq) prefetch(&tm_x1, ahead.tile * kTile, ahead.head);
-          prefetch(&tm_x2, ahead.tile * kTile, ahead.head);
-          prefetch(&tm_y1, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
-          prefetch(&tm_y2, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
-        }
         const int s1 = n % kY1, s2 = n % kY2;
         // Y1's last user is its tile's last MMA: dQ, or dK, which precedes the next tile's T2.
         if (n >= kY1 && !(kDq ? reuse_after(B_Y1_EMPTY + s1, (n / kY1 - 1) & 1) : reuse(B_T2_FULL, n - 2))) break;
@@ -815,6 +852,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive_expect_tx(bar(B_STAT + slot), kStatBytes);
           bulk_load(sbase + kSmStat + slot * kStatBytes, src, kStatBytes, bar(B_STAT + slot));
           ++nst;
+        }
+        if (it.first && ahead.next_busy()) {
+          const int y_head = kDq ? ahead.head / p.group : ahead.head * p.group;
+          if (!kDq) prefetch(&tm_x1, ahead.tile * kTile, ahead.head);
+          prefetch(&tm_x2, ahead.tile * kTile, ahead.head);
+          prefetch(&tm_y1, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
+          prefetch(&tm_y2, (ahead.t0 + (kDq ? ahead.skip : 0)) * kTile, y_head);
         }
       }
       if (*abort_flag) {
@@ -849,7 +893,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       named_bar_sync(id, threads);
       tc_fence_after();
     };
-    Tiles<kDq> it(p, slot);
+    Tiles it(p, slot);
     uint32_t items = 0;
     auto issue_t1 = [&](int slot, int parity) {
       if constexpr (kDq)
@@ -930,7 +974,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // for T2); then its rounds on the barriers whose release lets the issuer use them.  After
     // an abort the waits return at once and only the rounds are kept.
     int n1 = 0, n2 = 0, x1 = 0, x2 = 0;
-    Tiles<kDq> a(p, slot), c(p, slot);  // tiles whose T1 / T2 operands are next
+    Tiles a(p, slot), c(p, slot);  // tiles whose T1 / T2 operands are next
     auto t1_loaded = [&]() {
       if (!a.next()) return;
       if (lane == 0) {
@@ -953,7 +997,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       named_bar_sync(id, threads);
     };
-    Tiles<kDq> it(p, slot);
+    Tiles it(p, slot);
     bool have = it.next();
     if (have) {
       t1_loaded();

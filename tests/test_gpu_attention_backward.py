@@ -44,6 +44,10 @@ CASES = [
     (1, 1, 1, 3000, 3000, True),     # one head: both passes split along the sequence
     (1, 8, 1, 1500, 1200, True),
     (1, 4, 2, 130, 6000, False),
+    (1, 148, 148, 100, 100, True),   # causal pairs of tiles: a single tile per head,
+    (2, 74, 74, 129, 129, True),     # two,
+    (2, 74, 37, 300, 300, True),     # three, whose middle one has no partner,
+    (1, 37, 37, 1000, 1000, True),   # eight
 ]
 
 
