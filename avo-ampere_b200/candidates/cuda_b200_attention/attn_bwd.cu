@@ -18,9 +18,10 @@ int tiles_of(int rows) { return rows / kTile + (rows % kTile != 0); }
 
 template <bool kDq>
 auto kernel_of(bwd::Order order) {
-  return order == bwd::kPairs   ? bwd::attn_bwd_kernel<kDq, bwd::kPairs>
-         : order == bwd::kEqual ? bwd::attn_bwd_kernel<kDq, bwd::kEqual>
-                                : bwd::attn_bwd_kernel<kDq, bwd::kAny>;
+  return order == bwd::kPairs     ? bwd::attn_bwd_kernel<kDq, bwd::kPairs>
+         : order == bwd::kLongest ? bwd::attn_bwd_kernel<kDq, bwd::kLongest>
+         : order == bwd::kEqual   ? bwd::attn_bwd_kernel<kDq, bwd::kEqual>
+                                  : bwd::attn_bwd_kernel<kDq, bwd::kAny>;
 }
 
 // The kernels' shared-memory limit and register allocation, once per device.
@@ -38,6 +39,8 @@ int prepare_bwd(int* sm_count) {
                            reinterpret_cast<const void*>(kernel_of<true>(bwd::kAny)),
                            reinterpret_cast<const void*>(kernel_of<false>(bwd::kEqual)),
                            reinterpret_cast<const void*>(kernel_of<true>(bwd::kEqual)),
+                           reinterpret_cast<const void*>(kernel_of<false>(bwd::kLongest)),
+                           reinterpret_cast<const void*>(kernel_of<true>(bwd::kLongest)),
                            reinterpret_cast<const void*>(kernel_of<false>(bwd::kPairs)),
                            reinterpret_cast<const void*>(kernel_of<true>(bwd::kPairs))};
   for (const void* k : kernels) {
@@ -187,7 +190,7 @@ bwd::Order order_of(const Sizes& z, int sms) {
   const long long kv_more = kv % sms, q_more = q % sms;
   double most = kv_more + q_more > sms ? kv_us + q_us : std::max(kv_more > 0 ? kv_us : 0.0, q_more > 0 ? q_us : 0.0);
   most += kv / sms * kv_us + q / sms * q_us;
-  return most * 0.95 * sms < kv * kv_us + q * q_us ? bwd::kPairs : bwd::kAny;
+  return most * 0.95 * sms < kv * kv_us + q * q_us ? bwd::kPairs : bwd::kLongest;
 }
 
 void set_items(bwd::BwdParams& p, int heads, int tiles, int split, bwd::Order order) {
@@ -195,7 +198,7 @@ void set_items(bwd::BwdParams& p, int heads, int tiles, int split, bwd::Order or
   p.split_magic = ~0ull / p.split + 1;  // unused for 1
   const int rows = order == bwd::kPairs ? (tiles + 1) / 2 : tiles;
   p.item_count = static_cast<uint32_t>(heads) * static_cast<uint32_t>(rows) * p.split;
-  p.item_div = static_cast<uint32_t>(p.causal && order == bwd::kAny ? heads : rows);
+  p.item_div = static_cast<uint32_t>(p.causal && order != bwd::kPairs ? heads : rows);
   p.item_magic = ~0ull / p.item_div + 1;
 }
 

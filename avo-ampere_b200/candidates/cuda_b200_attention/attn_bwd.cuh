@@ -195,17 +195,18 @@ __device__ __forceinline__ uint32_t div_by(uint32_t w, uint32_t div, unsigned lo
   return div == 1 ? w : static_cast<uint32_t>(__umul64hi(w, magic));
 }
 
-// The order of the items, and what the kernel is compiled for.  The two cases with the most work
-// are simpler than the general one, and the softmax warps, short of registers, gain by that
-// (measured on B200, compiled for all cases / for its own: B4 H16 S4096 1547 / 1528 us; causal
-// B8 H16 S2048, in pairs in either, 545 / 520).
-//   kAny    waves over the grid in alternating directions.  Causal items are of different
-//           lengths: longest first, the same tile of all heads before the next tile.
-//   kEqual  (no mask, whole items) the same, heads one after the other.
-//   kPairs  (causal, equal lengths, whole items) heads one after the other, and each CTA takes
-//           the first and the last tile of a head, or the second and the last but one, and so
-//           on, which together are as long as any other pair.
-enum Order : int { kAny, kEqual, kPairs };
+// The order of the items, and what the kernel is compiled for.  Whole items without a mask, or
+// with one and equal lengths, are simpler than the general case, and the softmax warps, short
+// of registers, gain by that (measured on B200, compiled for all cases / for its own: B4 H16
+// S4096 1547 / 1528 us; causal B8 H16 S2048, in pairs in either, 545 / 520).
+//   kAny      waves over the grid in alternating directions.  Causal items are of different
+//             lengths: longest first, the same tile of all heads before the next tile.
+//   kEqual    (no mask, whole items) the same, heads one after the other.
+//   kLongest  (causal, equal lengths, whole items) as kAny.
+//   kPairs    (the same) heads one after the other, and each CTA takes the first and the last
+//             tile of a head, or the second and the last but one, and so on, which together are
+//             as long as any other pair.
+enum Order : int { kAny, kEqual, kLongest, kPairs };
 
 // One CTA's units in order (a stationary tile of one head, or a piece of its work).
 template <bool kDq, Order kOrder>
@@ -247,11 +248,11 @@ struct Items {
         const uint32_t unit = static_cast<uint32_t>(base) + ((r & 1) ? grid - 1 - cta : cta);
         ++r;
         if (unit >= p.item_count) continue;
-        const uint32_t w = kOrder == kEqual ? unit : div_by(unit, p.split, p.split_magic);
-        piece = kOrder == kEqual ? 0 : static_cast<int>(unit - w * p.split);
+        const uint32_t w = kOrder == kAny ? div_by(unit, p.split, p.split_magic) : unit;
+        piece = kOrder == kAny ? static_cast<int>(unit - w * p.split) : 0;
         const uint32_t quotient = div_by(w, p.item_div, p.item_magic);
         const int rest = static_cast<int>(w - quotient * p.item_div);
-        if (kOrder == kAny && p.causal) {
+        if (kOrder == kLongest || (kOrder == kAny && p.causal)) {
           head = rest;
           tile = kDq ? p.nq - 1 - static_cast<int>(quotient) : static_cast<int>(quotient);
         } else {
@@ -261,7 +262,7 @@ struct Items {
       }
       t0 = 0;
       skip = 0;
-      if constexpr (kOrder == kPairs) {
+      if constexpr (kOrder >= kLongest) {
         if (!kDq) t0 = tile;
         n = kDq ? tile + 1 : (p.nq - tile) * p.group;
         return true;
@@ -466,8 +467,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int row = threadIdx.x & 127;
     const uint32_t tBase = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * 16;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-    const bool causal = kOrder == kPairs || (kOrder == kAny && p.causal);
-    const int offset = kOrder == kPairs ? 0 : p.offset;
+    const bool causal = kOrder >= kLongest || (kOrder == kAny && p.causal);
+    const int offset = kOrder >= kLongest ? 0 : p.offset;
     uint32_t n = 0;
     float neg_lse = 0.f, neg_delta = 0.f;
     Tiles it(p, slot);
