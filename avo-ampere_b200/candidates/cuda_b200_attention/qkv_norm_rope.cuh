@@ -19,6 +19,11 @@
 // `heads_per_task` of its heads, four rows in flight at a time.  Everything is fp32 between
 // the load and one rounding to bf16.  The weights' gradients are summed per thread, then per
 // CTA, then over CTAs by a second kernel, each in a fixed order: equal inputs give equal bits.
+//
+// Memory bandwidth bounds both.  Measured on B200, B4 S4096 H16 Hkv4 (inputs not in L2): the
+// forward 35.9 us, 5.66 TB/s, against 31 at the rate of a plain copy; the gradient 58.7 us,
+// 4.9 TB/s, against 44.  What the gradient lacks is bytes in flight while its rows are computed
+// (about 50 instructions per 16 bytes of a row).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -90,6 +95,17 @@ __device__ __forceinline__ uint4 load_row(const __nv_bfloat16* row, const Column
   return make_uint4(a.x, a.y, b.x, b.y);
 }
 
+// The same on its way to 16 bytes of shared memory.
+template <bool kInterleaved>
+__device__ __forceinline__ void fetch_row(uint32_t to, const __nv_bfloat16* row, const Columns& c) {
+  if (kInterleaved) {
+    copy_async<16>(to, row + c.lo);
+  } else {
+    copy_async<8>(to, row + c.lo);
+    copy_async<8>(to + 8, row + c.hi);
+  }
+}
+
 template <bool kInterleaved>
 __device__ __forceinline__ void store_row(__nv_bfloat16* row, const Columns& c, uint4 v) {
   if (kInterleaved) {
@@ -157,23 +173,17 @@ __device__ __forceinline__ long long row_at(const RopeParams& p, const Task& t, 
   return ((static_cast<long long>(t.batch) * (t.kind == 0 ? p.heads : p.kv_heads) + h) * p.seq + t.s) * kRow;
 }
 
-// cos and sigma * sin of this lane's 8 columns (1 and 0 past the rotated part).
-template <bool kInterleaved>
-__device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, int l, float (&c)[8], float (&s)[8]) {
-  if (l * 8 >= p.rot) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      c[e] = 1.f;
-      s[e] = 0.f;
-    }
-    return;
-  }
-  const int half_rot = p.rot >> 1;
+// The table rows of a token, one per axis; whether one of them lies outside (then row 0).
+struct TableRows {
   long long row[kMaxAxes];
-  bool bad = false;
+  bool bad;
+};
+__device__ __forceinline__ TableRows table_rows(const RopeParams& p, const Task& t) {
+  TableRows rows;
+  rows.bad = false;
 #pragma unroll
   for (int a = 0; a < kMaxAxes; ++a) {
-    row[a] = 0;
+    rows.row[a] = 0;
     if (a < p.axes) {
       long long r = t.s;
       if (p.pos != nullptr) {
@@ -181,43 +191,87 @@ __device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, in
         r = p.pos64 ? __ldg(static_cast<const long long*>(p.pos) + at) : __ldg(static_cast<const int*>(p.pos) + at);
       }
       if (r < 0 || r >= p.table_rows) {
-        bad = true;
+        rows.bad = true;
         r = 0;
       }
-      row[a] = r;
+      rows.row[a] = r;
     }
   }
-  if (bad && t.valid && l == 0 && p.status != nullptr) atomicOr(p.status, kStatusPosition);
-  const int col = l * 4;  // this lane turns pairs col .. col + 3, table columns of the same index
-  float cc[4], ss[4];
-  auto row_of = [&](int f) {
-    long long r = row[0];
+  return rows;
+}
+
+// Where table column f of a token lies.
+__device__ __forceinline__ long long table_at(const RopeParams& p, const TableRows& rows, int f) {
+  long long r = rows.row[0];
 #pragma unroll
-    for (int a = 1; a < kMaxAxes; ++a)
-      if (a < p.axes && f >= p.end[a - 1]) r = row[a];
-    return r;
-  };
-  if (p.axes == 1) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row[0] * half_rot + col));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row[0] * half_rot + col));
-    cc[0] = a.x; cc[1] = a.y; cc[2] = a.z; cc[3] = a.w;
-    ss[0] = b.x; ss[1] = b.y; ss[2] = b.z; ss[3] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long at = row_of(col + i) * half_rot + col + i;
-      cc[i] = __ldg(p.cos + at);
-      ss[i] = __ldg(p.sin + at);
-    }
-  }
+  for (int a = 1; a < kMaxAxes; ++a)
+    if (a < p.axes && f >= p.end[a - 1]) r = rows.row[a];
+  return r * (p.rot >> 1) + f;
+}
+
+// cos and sigma * sin of this lane's 8 columns (1 and 0 past the rotated part), from those of
+// the 4 pairs that it turns.
+template <bool kInterleaved>
+__device__ __forceinline__ void spread_turn(bool turned, bool bad, const float4& cc4, const float4& ss4, float (&c)[8],
+                                            float (&s)[8]) {
   const float nan = __int_as_float(0x7fc00000);
+  const float cc[4] = {cc4.x, cc4.y, cc4.z, cc4.w}, ss[4] = {ss4.x, ss4.y, ss4.z, ss4.w};
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int i = kInterleaved ? e >> 1 : e & 3;
     const bool minus = kInterleaved ? (e & 1) == 0 : e < 4;
-    c[e] = bad ? nan : cc[i];
-    s[e] = bad ? nan : (minus ? -ss[i] : ss[i]);
+    c[e] = !turned ? 1.f : bad ? nan : cc[i];
+    s[e] = !turned ? 0.f : bad ? nan : (minus ? -ss[i] : ss[i]);
   }
+}
+
+template <bool kInterleaved>
+__device__ __forceinline__ void load_turn(const RopeParams& p, const Task& t, int l, float (&c)[8], float (&s)[8]) {
+  float4 cc = make_float4(1.f, 1.f, 1.f, 1.f), ss = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool bad = false;
+  const bool turned = l * 8 < p.rot;
+  if (turned) {
+    const TableRows rows = table_rows(p, t);
+    bad = rows.bad;
+    if (bad && t.valid && l == 0 && p.status != nullptr) atomicOr(p.status, kStatusPosition);
+    const int col = l * 4;  // this lane turns pairs col .. col + 3, table columns of the same index
+    if (p.axes == 1) {
+      const long long at = table_at(p, rows, col);
+      cc = __ldg(reinterpret_cast<const float4*>(p.cos + at));
+      ss = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+    } else {
+      float* const c4 = &cc.x;
+      float* const s4 = &ss.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long at = table_at(p, rows, col + i);
+        c4[i] = __ldg(p.cos + at);
+        s4[i] = __ldg(p.sin + at);
+      }
+    }
+  }
+  spread_turn<kInterleaved>(turned, bad, cc, ss, c, s);
+}
+
+// The same on their way to shared memory (nothing for lanes past the rotated part).
+__device__ __forceinline__ bool fetch_turn(const RopeParams& p, const Task& t, int l, uint32_t cos_to, uint32_t sin_to) {
+  if (l * 8 >= p.rot) return false;
+  const TableRows rows = table_rows(p, t);
+  if (rows.bad && t.valid && l == 0 && p.status != nullptr) atomicOr(p.status, kStatusPosition);
+  const int col = l * 4;
+  if (p.axes == 1) {
+    const long long at = table_at(p, rows, col);
+    copy_async<16>(cos_to, p.cos + at);
+    copy_async<16>(sin_to, p.sin + at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long at = table_at(p, rows, col + i);
+      copy_async<4>(cos_to + 4 * i, p.cos + at);
+      copy_async<4>(sin_to + 4 * i, p.sin + at);
+    }
+  }
+  return rows.bad;
 }
 
 // Index of the other half of value e of a lane.
@@ -350,10 +404,16 @@ __global__ void __launch_bounds__(kThreadsRope, kFwdCtasPerSm)
   }
 }
 
+// Groups of kUnroll rows go through shared memory: while a group is computed, the next one of
+// the warp (and the table rows, at a task's start) is on its way.  Every thread reads only what
+// it has fetched itself, so no barrier is needed.  (Measured as above: without this 64.2 us,
+// registers being full; with it 58.7; with 5 CTAs of 2, 3 or 4 rows a group 62.4, 69.4, 75.0.)
 template <bool kInterleaved>
 __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
     qkv_norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
   __shared__ float sums[kWarps][2][kRow];
+  __shared__ uint4 ring[2][2 * kUnroll][kThreadsRope];  // dy rows, then x rows, of a group
+  __shared__ float4 turns[2][2][kThreadsRope];
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, l = lane & 15, half = lane >> 4, warp = threadIdx.x >> 5;
@@ -379,44 +439,79 @@ __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
   };
   clear();
   int kind = 0;
-  for (long long task = static_cast<long long>(blockIdx.x) * kWarps + warp; task < p.tasks;
-       task += static_cast<long long>(gridDim.x) * kWarps) {
+
+  // The group that is fetched: its task's place, and how many of the task's rows are left.
+  long long task = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const __nv_bfloat16 *in = nullptr, *src = nullptr;
+  __nv_bfloat16* dst = nullptr;
+  int left = 0, next_kind = 0, tasks_begun = 0;
+  bool first = false, valid = false, bad = false;
+  auto begin_task = [&]() {
     const Task t = decode(p, task, half);
-    for (; kind < t.kind; ++kind)
-      if (norm && kind < 2) flush(kind);
     const int h_at = first_head(p, t.kind) + t.h0;
-    const __nv_bfloat16* src = p.qkv + t.batch * p.stride_b + t.s * p.stride_s + static_cast<long long>(h_at) * kRow;
-    __nv_bfloat16* dst =
-        p.dqkv + (static_cast<long long>(t.token) * (p.heads + 2 * p.kv_heads) + h_at) * kRow;
-    const __nv_bfloat16* in = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
-    int left = t.h1 - t.h0;
-    const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-    uint4 d[kUnroll], x[kUnroll];
-    auto load = [&]() {
+    src = p.qkv + t.batch * p.stride_b + t.s * p.stride_s + static_cast<long long>(h_at) * kRow;
+    dst = p.dqkv + (static_cast<long long>(t.token) * (p.heads + 2 * p.kv_heads) + h_at) * kRow;
+    in = (t.kind == 0 ? p.q : (t.kind == 1 ? p.k : p.v)) + row_at(p, t, t.h0);
+    left = t.h1 - t.h0;
+    next_kind = t.kind;
+    valid = t.valid;
+    first = true;
+    ++tasks_begun;
+    if (t.kind < 2) {
+      float4* const to = &turns[tasks_begun & 1][0][threadIdx.x];
+      bad = fetch_turn(p, t, l, smem_addr(to), smem_addr(to + kThreadsRope));
+    }
+  };
+  auto fetch = [&](int stage) {
+    const uint32_t to = smem_addr(&ring[stage][0][threadIdx.x]);
+    constexpr uint32_t kNext = kThreadsRope * sizeof(uint4);
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        // (Rows past the run: a zero gradient on ones.)
-        d[i] = i < left ? load_row<kInterleaved>(in + i * step, col) : make_uint4(0u, 0u, 0u, 0u);
-        x[i] = i < left && t.kind < 2 && norm ? load_row<kInterleaved>(src + i * kRow, col) : ones;
-      }
-      in += kUnroll * step;
-      src += kUnroll * kRow;
-    };
-    load();
-    if (t.kind == 2) {
-      for (; left > 0; left -= kUnroll, dst += kUnroll * kRow) {
-        if (left < t.h1 - t.h0) load();
+    for (int i = 0; i < kUnroll; ++i) {
+      if (i >= left) break;
+      fetch_row<kInterleaved>(to + i * kNext, in + i * step, col);
+      if (next_kind < 2 && norm) fetch_row<kInterleaved>(to + (kUnroll + i) * kNext, src + i * kRow, col);
+    }
+  };
+  const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  uint64_t c2[4], s2[4], w2[4];
+  bool more = task < p.tasks;
+  if (more) {
+    begin_task();
+    fetch(0);
+  }
+  copy_async_commit();
+  for (int stage = 0; more; stage ^= 1) {
+    // This group; then the next one is fetched.
+    __nv_bfloat16* const out = dst;
+    const int rows = left, this_kind = next_kind, turn = tasks_begun & 1;
+    const bool begun = first, store = valid, nan = bad;
+    first = false;
+    left -= kUnroll;
+    in += kUnroll * step;
+    src += kUnroll * kRow;
+    dst += kUnroll * kRow;
+    if (left <= 0) {
+      task += static_cast<long long>(gridDim.x) * kWarps;
+      more = task < p.tasks;
+      if (more) begin_task();
+    }
+    if (more) fetch(stage ^ 1);
+    copy_async_commit();
+    copy_async_wait<1>();
+    const uint4* const from = &ring[stage][0][threadIdx.x];
+    if (this_kind == 2) {
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i)
-          if (i < left && t.valid) store_row<kInterleaved>(dst + i * kRow, col, d[i]);
-      }
+      for (int i = 0; i < kUnroll; ++i)
+        if (i < rows && store) store_row<kInterleaved>(out + i * kRow, col, from[i * kThreadsRope]);
       continue;
     }
-    uint64_t c2[4], s2[4], w2[4];
-    {
+    if (begun) {
+      for (; kind < this_kind; ++kind)
+        if (norm) flush(kind);
       float c[8], s[8], w[8];
-      load_turn<kInterleaved>(p, t, l, c, s);
-      if (norm) load_weights(t.kind == 0 ? p.q_weight : p.k_weight, p.weight_bf16, col, w);
+      const float4* const at = &turns[turn][0][threadIdx.x];
+      spread_turn<kInterleaved>(col.turned, nan, at[0], at[kThreadsRope], c, s);
+      if (norm) load_weights(this_kind == 0 ? p.q_weight : p.k_weight, p.weight_bf16, col, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         c2[i] = f2_pack(c[2 * i], c[2 * i + 1]);
@@ -424,38 +519,39 @@ __global__ void __launch_bounds__(kThreadsRope, kBwdCtasPerSm)
         w2[i] = norm ? f2_pack(w[2 * i], w[2 * i + 1]) : 0;
       }
     }
-    for (; left > 0; left -= kUnroll, dst += kUnroll * kRow) {
-      if (left < t.h1 - t.h0) load();
+    const float live = store ? 1.f : 0.f;
+    const uint64_t live2 = f2_pack(live, live);
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        uint64_t g[4], o[4], turned[4];
-        unpack4(d[i], g);
-        others4<kInterleaved>(d[i], g, o);
+    for (int i = 0; i < kUnroll; ++i) {
+      // (Rows past the run: a zero gradient on ones.)
+      const uint4 d = i < rows ? from[i * kThreadsRope] : make_uint4(0u, 0u, 0u, 0u);
+      uint64_t g[4], o[4], turned[4];
+      unpack4(d, g);
+      others4<kInterleaved>(d, g, o);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) turned[e] = f2_fma(o[e], s2[e], f2_mul(g[e], c2[e]));
-        if (norm) {
-          uint64_t f[4], gw[4];
-          unpack4(x[i], f);
-          // The two sums of the row are taken side by side: mean(g w x_hat) = r mean(g w x).
+      for (int e = 0; e < 4; ++e) turned[e] = f2_fma(o[e], s2[e], f2_mul(g[e], c2[e]));
+      if (norm) {
+        const uint4 x = i < rows ? from[(kUnroll + i) * kThreadsRope] : ones;
+        uint64_t f[4], gw[4];
+        unpack4(x, f);
+        // The two sums of the row are taken side by side: mean(g w x_hat) = r mean(g w x).
 #pragma unroll
-          for (int e = 0; e < 4; ++e) gw[e] = f2_mul(turned[e], w2[e]);
-          const float sq = row_dot(f, f), dot = row_dot(gw, f);
-          const float r = rsqrtf(sq * (1.f / kRow) + p.eps);
-          const float m = -dot * (1.f / kRow) * r;
-          const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
-          const float live = t.valid ? 1.f : 0.f;
-          const uint64_t live2 = f2_pack(live, live);
+        for (int e = 0; e < 4; ++e) gw[e] = f2_mul(turned[e], w2[e]);
+        const float sq = row_dot(f, f), dot = row_dot(gw, f);
+        const float r = rsqrtf(sq * (1.f / kRow) + p.eps);
+        const float m = -dot * (1.f / kRow) * r;
+        const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[e] = f2_mul(f[e], r2);  // x_hat
-            dw[e] = f2_fma(f2_mul(turned[e], live2), f[e], dw[e]);
-            turned[e] = f2_mul(r2, f2_fma(f[e], m2, gw[e]));
-          }
+        for (int e = 0; e < 4; ++e) {
+          f[e] = f2_mul(f[e], r2);  // x_hat
+          dw[e] = f2_fma(f2_mul(turned[e], live2), f[e], dw[e]);
+          turned[e] = f2_mul(r2, f2_fma(f[e], m2, gw[e]));
         }
-        if (i < left && t.valid) store_row<kInterleaved>(dst + i * kRow, col, pack4(turned));
       }
+      if (i < rows && store) store_row<kInterleaved>(out + i * kRow, col, pack4(turned));
     }
   }
+  copy_async_wait<0>();
   if (!norm) return;
   for (; kind < 2; ++kind) flush(kind);
   __syncthreads();

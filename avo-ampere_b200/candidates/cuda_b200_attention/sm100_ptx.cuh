@@ -107,6 +107,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // Two packed fp32 pairs from shared memory (16-byte aligned).
+// Per-thread asynchronous copies to shared memory, both addresses aligned to their size; a
+// commit closes a group, wait<n> leaves at most the last n groups in flight.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kGroups>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kGroups) : "memory");
+}
+
 // The multiprocessor this thread runs on.
 __device__ __forceinline__ uint32_t sm_id() {
   uint32_t id;
