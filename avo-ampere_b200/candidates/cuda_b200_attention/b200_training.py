@@ -43,6 +43,7 @@ b = _binding()
 HEAD_DIM = b.HEAD_DIM
 
 
+@functools.cache
 def _torch():
     import torch
 
@@ -92,10 +93,10 @@ def _attention_shape(q, k, v) -> tuple[int, int, int, int, int]:
     index = q.get_device()
     if not (_plain(q, bf16, index) and _plain(k, bf16, index) and _plain(v, bf16, index)):
         _check_tensors((("q", q), ("k", k), ("v", v)), bf16)
-    qs, ks = q.shape, k.shape
-    if len(qs) != 4 or len(ks) != 4 or v.dim() != 4:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise RuntimeError("q, k, and v must have shape (batch, heads, seq, dim)")
-    if ks != v.shape:
+    if ks != vs:
         raise RuntimeError("k and v must have the same shape")
     batch, heads, seq_q, dim = qs
     kv_batch, kv_heads, seq_kv, kv_dim = ks
@@ -241,17 +242,19 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
         _check_tensors((("dout", dout), ("out", out)), torch.bfloat16, q.device)
     if not _plain(lse, torch.float32, index):
         _check_tensors((("lse", lse),), torch.float32, q.device)
-    if dout.shape != q.shape or out.shape != q.shape:
-        raise RuntimeError(f"{'out' if dout.shape == q.shape else 'dout'} must have the shape of q")
-    if lse.shape != q.shape[:3]:
+    shape = (batch, heads, seq_q, HEAD_DIM)
+    if dout.shape != shape or out.shape != shape:
+        raise RuntimeError(f"{'out' if dout.shape == shape else 'dout'} must have the shape of q")
+    if lse.shape != shape[:3]:
         raise RuntimeError("lse must have shape (batch, heads, seq)")
-    given = [(name, t, like) for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)) if t is not None]
-    for i, (name, t, like) in enumerate(given):
-        _check_tensors(((name, t),), torch.bfloat16, q.device)
-        if t.shape != like.shape:
-            raise RuntimeError(f"{name} must have the shape of {name[1:]}")
-        if any(_overlap(t, other) for other in (dout, q, k, v, out, lse, *(g[1] for g in given[:i]))):
-            raise RuntimeError(f"{name} must not overlap another tensor of the call")
+    if dq is not None or dk is not None or dv is not None:
+        given = [(name, t, like) for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)) if t is not None]
+        for i, (name, t, like) in enumerate(given):
+            _check_tensors(((name, t),), torch.bfloat16, q.device)
+            if t.shape != like.shape:
+                raise RuntimeError(f"{name} must have the shape of {name[1:]}")
+            if any(_overlap(t, other) for other in (dout, q, k, v, out, lse, *(g[1] for g in given[:i]))):
+                raise RuntimeError(f"{name} must not overlap another tensor of the call")
     grads = (torch.empty_like(q) if dq is None else dq, torch.empty_like(k) if dk is None else dk,
              torch.empty_like(v) if dv is None else dv)
     with _on(index):
@@ -270,9 +273,17 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
 MAX_AXES = 4
 
 
+@functools.lru_cache(maxsize=64)
+def _section_array(counts: tuple[int, ...], pairs: int):
+    """(axes, the C array) of checked section counts."""
+    if not 1 <= len(counts) <= MAX_AXES or any(n < 0 for n in counts) or sum(counts) != pairs:
+        raise RuntimeError(f"sections must be 1 to {MAX_AXES} counts that sum to rotary_dim / 2")
+    return len(counts), (ctypes.c_int * len(counts))(*counts)
+
+
 def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved):
-    """Checks the arguments both directions share; (batch, seq, device arguments of the C
-    calls from `batch` to `eps`, what they point to)."""
+    """Checks the arguments both directions share; (batch, seq, the C calls' arguments for qkv,
+    those from `batch` to `eps`, what they point to)."""
     torch = _torch()
     if not qkv.is_cuda:
         raise RuntimeError("qkv must be a CUDA tensor")
@@ -280,78 +291,76 @@ def _rope_args(qkv, heads: int, kv_heads: int, cos, sin, q_weight, k_weight, pos
         raise RuntimeError("qkv must be bf16")
     if heads < 0 or kv_heads < 0:
         raise RuntimeError("the numbers of heads must not be negative")
-    if qkv.dim() != 4 or qkv.shape[2] != heads + 2 * kv_heads or qkv.shape[3] != HEAD_DIM:
+    shape = qkv.shape
+    if len(shape) != 4 or shape[2] != heads + 2 * kv_heads or shape[3] != HEAD_DIM:
         raise RuntimeError(f"qkv must have shape (batch, seq, heads + 2 * kv_heads, {HEAD_DIM})")
-    batch, seq, all_heads, _ = qkv.shape
-    _, _, head_stride, last_stride = qkv.stride()
+    batch, seq, all_heads, _ = shape
+    batch_stride, token_stride, head_stride, last_stride = qkv.stride()
     if (last_stride != 1 or (all_heads > 1 and head_stride != HEAD_DIM)) and qkv.numel():
         raise RuntimeError("the heads of a token of qkv must be contiguous")
+    # (A dimension of one element has no stride to speak of.)
+    place = (qkv.data_ptr(), batch_stride if batch > 1 else 0, token_stride if seq > 1 else 0)
     index = qkv.get_device()
     if not (_plain(cos, torch.float32, index) and _plain(sin, torch.float32, index)):
         _check_tensors((("cos", cos), ("sin", sin)), torch.float32, qkv.device)
-    if cos.dim() != 2 or cos.shape != sin.shape:
+    table = cos.shape
+    if len(table) != 2 or table != sin.shape:
         raise RuntimeError("cos and sin must have the same shape (positions, rotary_dim / 2)")
-    table_rows, pairs = cos.shape
+    table_rows, pairs = table
     rotary = 2 * pairs
     if rotary == 0 or rotary > HEAD_DIM or rotary % 16 != 0:
         raise RuntimeError(f"rotary_dim must be a multiple of 16 up to {HEAD_DIM}")
     if (q_weight is None) != (k_weight is None):
         raise RuntimeError("q_weight and k_weight must be given together")
+    weights_at, weights_bf16 = (None, None), 0
     if q_weight is not None:
         dtype = q_weight.dtype
         if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise RuntimeError("q_weight must be fp32 or bf16")
         if not (_plain(q_weight, dtype, index) and _plain(k_weight, dtype, index)):
             _check_tensors((("q_weight", q_weight), ("k_weight", k_weight)), dtype, qkv.device)
-        if q_weight.dim() != 1 or q_weight.shape != k_weight.shape or q_weight.numel() != HEAD_DIM:
+        if q_weight.shape != (HEAD_DIM,) or k_weight.shape != (HEAD_DIM,):
             raise RuntimeError(f"q_weight and k_weight must have shape ({HEAD_DIM},)")
+        weights_at, weights_bf16 = (q_weight.data_ptr(), k_weight.data_ptr()), int(dtype is torch.bfloat16)
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise RuntimeError("eps must not be negative")
-    axes, section_array, strides = 1, None, (0, 0, 0)
+    axes, section_array, sections_at, strides, positions_at, wide = 1, None, None, (0, 0, 0), None, 0
     if sections is not None:
-        sections = [int(n) for n in sections]
-        axes = len(sections)
-        if not 1 <= axes <= MAX_AXES or any(n < 0 for n in sections) or sum(sections) != rotary // 2:
-            raise RuntimeError(f"sections must be 1 to {MAX_AXES} counts that sum to rotary_dim / 2")
+        axes, section_array = _section_array(tuple(map(int, sections)), pairs)
         if positions is None:
             raise RuntimeError("sections need positions")
-        section_array = (ctypes.c_int * axes)(*sections)
+        sections_at = ctypes.addressof(section_array)
     if positions is None:
         if seq > table_rows:
             raise RuntimeError("cos and sin have fewer rows than the sequence has tokens")
     else:
         if not positions.is_cuda or positions.get_device() != index:
             raise RuntimeError("positions must be on the device of qkv")
-        if positions.dtype is not torch.int32 and positions.dtype is not torch.int64:
+        wide = int(positions.dtype is torch.int64)
+        if not wide and positions.dtype is not torch.int32:
             raise RuntimeError("positions must be int32 or int64")
-        shape = positions.shape if sections is None else positions.shape[1:]
-        if shape != (batch, seq) and shape != (seq,) or (sections is not None and positions.shape[0] != axes):
+        shape = positions.shape
+        lead_ok = sections is None or shape[:1] == (axes,)
+        if sections is not None:
+            shape = shape[1:]
+        if shape != (batch, seq) and shape != (seq,) or not lead_ok:
             lead = "" if sections is None else "axes, "
             raise RuntimeError(f"positions must have shape ({lead}seq) or ({lead}batch, seq)")
         if table_rows == 0 and positions.numel():
             raise RuntimeError("cos and sin have no rows")
         at = positions.stride()
         strides = (at[0] if sections is not None else 0, at[-2] if len(shape) == 2 else 0, at[-1])
-    args = [batch, seq, heads, kv_heads, HEAD_DIM,
-            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-            int(q_weight is not None and q_weight.dtype == torch.bfloat16), cos.data_ptr(), sin.data_ptr(),
-            table_rows, rotary, 1 if interleaved else 0, None if positions is None else positions.data_ptr(),
-            int(positions is not None and positions.dtype == torch.int64), *strides, axes,
-            None if section_array is None else ctypes.addressof(section_array), eps]
-    return batch, seq, args, section_array
-
-
-def _qkv_strides(qkv) -> tuple[int, int]:
-    """Batch and token stride (a dimension of one element has no stride to speak of)."""
-    (batch, seq, _, _), (at, by, _, _) = qkv.shape, qkv.stride()
-    return (at if batch > 1 else 0), (by if seq > 1 else 0)
+        positions_at = positions.data_ptr()
+    args = (batch, seq, heads, kv_heads, HEAD_DIM, *weights_at, weights_bf16, cos.data_ptr(), sin.data_ptr(),
+            table_rows, rotary, 1 if interleaved else 0, positions_at, wide, *strides, axes, sections_at, eps)
+    return batch, seq, place, args, section_array
 
 
 def _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps, interleaved):
     torch = _torch()
-    batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
-                                        interleaved)
+    batch, seq, place, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections,
+                                               eps, interleaved)
     q = qkv.new_empty((batch, heads, seq, HEAD_DIM))
     k = qkv.new_empty((batch, kv_heads, seq, HEAD_DIM))
     v = torch.empty_like(k)
@@ -360,7 +369,7 @@ def _norm_rope(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, se
     b.load_library()
     index = qkv.get_device()
     with _on(index):
-        code = b.call_entry(2, qkv.data_ptr(), *_qkv_strides(qkv), q.data_ptr(), k.data_ptr(), v.data_ptr(), *args,
+        code = b.call_entry(2, *place, q.data_ptr(), k.data_ptr(), v.data_ptr(), *args,
                             b.status_address(index), b._raw_stream(index))
     del keep
     b._check(code, "avo_b200_qkv_norm_rope")
@@ -379,27 +388,27 @@ def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight
     if not (_plain(dq, torch.bfloat16, index) and _plain(dk, torch.bfloat16, index)
             and _plain(dv, torch.bfloat16, index)):
         _check_tensors((("dq", dq), ("dk", dk), ("dv", dv)), torch.bfloat16, qkv.device)
-    if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape:
+    dq_shape, dk_shape = dq.shape, dk.shape
+    if len(dq_shape) != 4 or len(dk_shape) != 4 or dk_shape != dv.shape:
         raise RuntimeError("dq, dk and dv must have shape (batch, heads, seq, dim), dk and dv the same")
-    heads, kv_heads = dq.shape[1], dk.shape[1]
-    batch, seq, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections, eps,
-                                        interleaved)
-    if tuple(dq.shape) != (batch, heads, seq, HEAD_DIM) or tuple(dk.shape) != (batch, kv_heads, seq, HEAD_DIM):
+    heads, kv_heads = dq_shape[1], dk_shape[1]
+    batch, seq, place, args, keep = _rope_args(qkv, heads, kv_heads, cos, sin, q_weight, k_weight, positions, sections,
+                                               eps, interleaved)
+    if dq_shape != (batch, heads, seq, HEAD_DIM) or dk_shape != (batch, kv_heads, seq, HEAD_DIM):
         raise RuntimeError("dq, dk and dv must match qkv's batch and sequence")
     dqkv = qkv.new_empty(qkv.shape)
     b.load_library()
-    index = qkv.get_device()
     with _on(index):
-        weights, scratch, size = (None, None), None, 0
+        weights, scratch, more = (None, None), None, (None, 0)
+        weights_at = weights
         if q_weight is not None:
             weights = cos.new_empty((2, HEAD_DIM)).unbind()
+            weights_at = (weights[0].data_ptr(), weights[1].data_ptr())
             size = _rope_scratch_bytes(index)
             scratch = qkv.new_empty(size, dtype=torch.uint8)
-        code = b.call_entry(
-            3, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), *_qkv_strides(qkv), dqkv.data_ptr(),
-            None if q_weight is None else weights[0].data_ptr(), None if q_weight is None else weights[1].data_ptr(),
-            *args, None if scratch is None else scratch.data_ptr(), size, b.status_address(index),
-            b._raw_stream(index))
+            more = (scratch.data_ptr(), size)
+        code = b.call_entry(3, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *place, dqkv.data_ptr(), *weights_at, *args,
+                            *more, b.status_address(index), b._raw_stream(index))
     del keep
     b._check(code, "avo_b200_qkv_norm_rope_bwd")
     return (dqkv, *weights)
@@ -470,7 +479,7 @@ def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=
     Such a call cannot be captured in a CUDA graph: capture the call under
     ``torch.no_grad()`` and ``qkv_norm_rope_backward``."""
     torch = _torch()
-    sections = None if sections is None else tuple(int(n) for n in sections)
+    sections = None if sections is None else tuple(map(int, sections))
     heads, kv_heads, interleaved = int(num_heads), int(num_kv_heads), bool(interleaved)
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise RuntimeError("qkv_norm_rope has no gradient for cos and sin: detach them")
