@@ -485,14 +485,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       named_bar_sync(bar_tile(kRoundDs, n), kDsThreads<kDq>);
     };
-    // dQ: the statistics of this row in the item after the current one, loaded an item ahead.
+    // dQ: the statistics of this row in the item after the current one, loaded an item ahead
+    // (from L2, where the launch before dK/dV has left them: this launch has not waited for it).
     Items ahead(p, slot);
     float next_lse = 0.f, next_delta = 0.f;
     auto load_stats = [&]() {
       if (!ahead.next_busy()) return;
       const float* st = p.stats + (static_cast<long long>(ahead.head) * p.nq + ahead.tile) * (2 * kTile);
-      next_lse = __ldg(st + row);
-      next_delta = __ldg(st + kTile + row);
+      next_lse = __ldcg(st + row);
+      next_delta = __ldcg(st + kTile + row);
     };
     if (kDq) load_stats();
     const uint32_t tT1 = tBase + kColT1, tT2 = tBase + kColT2;
