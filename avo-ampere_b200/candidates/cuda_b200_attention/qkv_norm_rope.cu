@@ -66,7 +66,8 @@ int fill(rope::RopeParams& p, const void* qkv, long long stride_b, long long str
 
 // Heads per task: a task reads its token's table rows once, so more heads share them, but
 // there have to be enough tasks (warps) to keep every multiprocessor's memory queue full.
-void split_heads(rope::RopeParams& p, int sms) {
+// False where they cannot be counted in 31 bits.
+bool split_heads(rope::RopeParams& p, int sms) {
   const long long pairs = (static_cast<long long>(p.tokens) + 1) / 2;
   auto segs = [](int heads, int per) { return (heads + per - 1) / per; };
   int per = 16;
@@ -74,9 +75,16 @@ void split_heads(rope::RopeParams& p, int sms) {
   p.heads_per_task = per;
   p.segs_q = segs(p.heads, per);
   p.segs_kv = segs(p.kv_heads, per);
-  p.q_tasks = pairs * p.segs_q;
-  p.k_tasks = pairs * p.segs_kv;
+  const long long q_tasks = pairs * p.segs_q, k_tasks = pairs * p.segs_kv;
+  if (q_tasks + 2 * k_tasks > INT_MAX) return false;  // (about 10^13 bytes)
+  p.q_tasks = static_cast<uint32_t>(q_tasks);
+  p.k_tasks = static_cast<uint32_t>(k_tasks);
   p.tasks = p.q_tasks + 2 * p.k_tasks;
+  auto magic = [](int x) { return x > 0 ? ~0ull / static_cast<unsigned>(x) + 1 : 0; };  // unused for 1
+  p.segs_q_magic = magic(p.segs_q);
+  p.segs_kv_magic = magic(p.segs_kv);
+  p.seq_magic = magic(p.seq);
+  return true;
 }
 
 long long ctas_for(long long tasks) { return (tasks + rope::kWarps - 1) / rope::kWarps; }
@@ -110,9 +118,8 @@ extern "C" int avo_b200_qkv_norm_rope(const void* qkv, long long batch_stride, l
   p.q = static_cast<__nv_bfloat16*>(q);
   p.k = static_cast<__nv_bfloat16*>(k);
   p.v = static_cast<__nv_bfloat16*>(v);
-  split_heads(p, sms);
+  if (!split_heads(p, sms)) return AVO_B200_EINVAL;
   const long long ctas = ctas_for(p.tasks);
-  if (ctas > INT_MAX) return AVO_B200_EINVAL;
   auto* kernel = interleaved ? rope::qkv_norm_rope_kernel<true> : rope::qkv_norm_rope_kernel<false>;
   if (!host::launch_early(kernel, static_cast<unsigned>(ctas), rope::kThreadsRope, 0,
                           static_cast<cudaStream_t>(stream), p))
@@ -165,7 +172,7 @@ extern "C" int avo_b200_qkv_norm_rope_bwd(const void* dq, const void* dk, const 
   p.k = static_cast<__nv_bfloat16*>(const_cast<void*>(dk));
   p.v = static_cast<__nv_bfloat16*>(const_cast<void*>(dv));
   p.dqkv = static_cast<__nv_bfloat16*>(dqkv);
-  split_heads(p, sms);
+  if (!split_heads(p, sms)) return AVO_B200_EINVAL;
   long long ctas = ctas_for(p.tasks);
   const long long most = static_cast<long long>(sms) * rope::kBwdCtasPerSm;
   if (ctas > most) ctas = most;
@@ -175,7 +182,7 @@ extern "C" int avo_b200_qkv_norm_rope_bwd(const void* dq, const void* dk, const 
   p.partial = static_cast<float*>(workspace);
   auto* kernel = interleaved ? rope::qkv_norm_rope_bwd_kernel<true> : rope::qkv_norm_rope_bwd_kernel<false>;
   if (!host::launch_early(kernel, static_cast<unsigned>(ctas), rope::kThreadsRope, 0, st, p)) return AVO_B200_ELAUNCH;
-  if (norm && !host::launch_early(rope::weight_grad_kernel, 2 * rope::kRow / 32, 1024u, 0, st,
+  if (norm && !host::launch_early(rope::weight_grad_kernel, 2 * rope::kRow / rope::kSumCols, 1024u, 0, st,
                                   static_cast<const float*>(p.partial), static_cast<int>(ctas), dq_weight, dk_weight))
     return AVO_B200_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? AVO_B200_OK : AVO_B200_ELAUNCH;
