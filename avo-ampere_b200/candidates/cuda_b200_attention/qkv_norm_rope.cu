@@ -64,9 +64,11 @@ int fill(rope::RopeParams& p, const void* qkv, long long stride_b, long long str
   return AVO_B200_OK;
 }
 
-// Heads per task: a task reads its token's table rows once, so more heads share them, but
-// there have to be enough tasks (warps) to keep every multiprocessor's memory queue full.
-// False where they cannot be counted in 31 bits.
+// Heads per task: a task reads its token's table rows once and a contiguous run of memory, so
+// that more heads share them, but there have to be enough tasks (warps) to keep every
+// multiprocessor's memory queue full.  (Measured on B200, B4 S4096 H16 Hkv4, up to 16 / 12 / 8 / 4
+// heads: forward 35.0 / 37.4 / 35.7 / 39.9 us, gradient 56.8 / 64.3 / 59.8 / 64.3.)  False where
+// the tasks cannot be counted in 31 bits.
 bool split_heads(rope::RopeParams& p, int sms) {
   const long long pairs = (static_cast<long long>(p.tokens) + 1) / 2;
   auto segs = [](int heads, int per) { return (heads + per - 1) / per; };

@@ -21,8 +21,8 @@
 // CTA, then over CTAs by a second kernel, each in a fixed order: equal inputs give equal bits.
 //
 // Memory bandwidth bounds both.  Measured on B200, B4 S4096 H16 Hkv4 (inputs not in L2): the
-// forward 35.9 us, 5.66 TB/s, against 31 at the rate of a plain copy; the gradient 58.7 us,
-// 4.9 TB/s, against 44.  The gradient's issue slots are 60 % busy with a quarter of the warps
+// forward 34.8 us, 5.85 TB/s, against 31 at the rate of a plain copy; the gradient 56.7 us,
+// 5.07 TB/s, against 44.  The gradient's issue slots are 60 % busy with a quarter of the warps
 // resident (its registers), so computing and fetching do not overlap fully.
 #pragma once
 
