@@ -301,12 +301,11 @@ extern "C" int avo_b200_attn_bwd(const void* dout, const void* q, const void* k,
   const unsigned kv_grid = static_cast<unsigned>(kv_units > sms ? sms : kv_units);
   const unsigned q_grid = static_cast<unsigned>(q_units > sms ? sms : q_units);
 
-  const long long rows = static_cast<long long>(z.q_heads) * p.nq * kTile;
-  const long long blocks = rows / 16;
+  const long long blocks = static_cast<long long>(z.q_heads) * p.nq * (kTile / bwd::kStatBlockRows);
   if (blocks > INT_MAX) return AVO_B200_EINVAL;
   if (!host::launch_early(bwd::stats_kernel, static_cast<unsigned>(blocks), 256u, 0, st,
-                          static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse,
-                          stats, rows, z.seq_q, p.nq, claims))
+                          static_cast<const uint4*>(dout), static_cast<const uint4*>(out), lse, stats, z.seq_q, p.nq,
+                          claims))
     return AVO_B200_ELAUNCH;
   set_items(p, z.kv_heads, z.nkv, z.split_kv, order);
   p.claims = by_place ? claims : nullptr;
