@@ -186,24 +186,26 @@ int prepare_device(int* sm_count = nullptr) {
     if (dev < kMaxDevices) g_device_state[dev] = -1;
     return AVO_B200_ENODEV;
   }
-  if (cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
-          cudaSuccess ||
-      cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
-          cudaSuccess) {
-    (void)cudaGetLastError();
-    return AVO_B200_ELAUNCH;
-  }
+  const void* kernels[] = {reinterpret_cast<const void*>(attn_fwd_kernel<false, 3>),
+                           reinterpret_cast<const void*>(attn_fwd_kernel<true, 3>),
+                           reinterpret_cast<const void*>(attn_fwd_kernel<false, 5>),
+                           reinterpret_cast<const void*>(attn_fwd_kernel<true, 5>)};
+  for (const void* k : kernels)
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return AVO_B200_ELAUNCH;
+    }
   // The kernel rebalances registers between warpgroups with setmaxnreg, which only
   // works out if the launch allocation is exactly the one the split was computed for;
   // otherwise an increase could wait forever.  Refuse to launch in that case.
-  cudaFuncAttributes attr{}, attr_t{};
-  if (cudaFuncGetAttributes(&attr, attn_fwd_kernel<false>) != cudaSuccess ||
-      cudaFuncGetAttributes(&attr_t, attn_fwd_kernel<true>) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return AVO_B200_ELAUNCH;
+  for (const void* k : kernels) {
+    cudaFuncAttributes attr{};
+    if (cudaFuncGetAttributes(&attr, k) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return AVO_B200_ELAUNCH;
+    }
+    if (attr.numRegs != static_cast<int>(kRegsLaunch)) return AVO_B200_EREGS;
   }
-  if (attr.numRegs != static_cast<int>(kRegsLaunch) || attr_t.numRegs != static_cast<int>(kRegsLaunch))
-    return AVO_B200_EREGS;
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
     (void)cudaGetLastError();
@@ -320,7 +322,8 @@ const PlanEntry& cached_plan(int num_bh, int seq_q, int seq_kv, int causal, long
 int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int num_bh,
                int seq_q, int seq_kv, int head_dim, long long q_hs, long long kv_hs, long long o_hs,
                long long lse_hs, int causal, float scale, long long q_pos0, long long kv_pos0,
-               int* status, void* stream, void* workspace = nullptr, size_t workspace_bytes = 0, int kv_group = 1) {
+               int* status, void* stream, void* workspace = nullptr, size_t workspace_bytes = 0, int kv_group = 1,
+               bool fine = false) {
   if (q == nullptr || k == nullptr || v == nullptr || o == nullptr) return AVO_B200_EINVAL;
   if (head_dim != kHeadDim || num_bh < 0 || seq_q < 0 || seq_kv < 0) return AVO_B200_EINVAL;
   if (!(scale > 0.f) || !std::isfinite(scale)) return AVO_B200_EINVAL;
@@ -400,20 +403,20 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, attn_fwd_kernel<false>, tm_q, tm_k, tm_v, p, TableParam<false>{0}) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, fine ? attn_fwd_kernel<false, 5> : attn_fwd_kernel<false, 3>, tm_q, tm_k, tm_v, p, TableParam<false>{0}) != cudaSuccess) {
       (void)cudaGetLastError();
       return AVO_B200_ELAUNCH;
     }
   } else if (plan.mode == sched::kTable) {
-    attn_fwd_kernel<true><<<static_cast<unsigned>(grid), kThreads, kSmemBytes, st>>>(tm_q, tm_k, tm_v, p,
-                                                                                      entry.table);
+    auto* kernel = fine ? attn_fwd_kernel<true, 5> : attn_fwd_kernel<true, 3>;
+    kernel<<<static_cast<unsigned>(grid), kThreads, kSmemBytes, st>>>(tm_q, tm_k, tm_v, p, entry.table);
   } else {
     // Split pieces: a CTA that merges an item waits for its neighbours' continuation
     // pieces, so every CTA must be resident at once; a cooperative launch guarantees it
     // (or fails to launch).
     TableParam<false> none{0};
     void* args[] = {&tm_q, &tm_k, &tm_v, &p, &none};
-    if (cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(attn_fwd_kernel<false>), dim3(grid),
+    if (cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(fine ? attn_fwd_kernel<false, 5> : attn_fwd_kernel<false, 3>), dim3(grid),
                                     dim3(kThreads), args, kSmemBytes, st) != cudaSuccess) {
       (void)cudaGetLastError();
       return AVO_B200_ELAUNCH;
@@ -505,7 +508,7 @@ extern "C" int avo_b200_attn_fwd_grouped(const void* q, const void* k, const voi
   // With a mask, query row i sits at position seq_kv - seq_q + i: the last query sees every key.
   return launch_fwd(q, k, v, o, lse, static_cast<int>(pairs), seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim,
                     qhs, seq_q, causal, softmax_scale, causal ? static_cast<long long>(seq_kv) - seq_q : 0, 0,
-                    status_dev, stream, workspace, workspace_bytes, group);
+                    status_dev, stream, workspace, workspace_bytes, group, true);
 }
 
 extern "C" int avo_b200_attn_workspace_size(size_t* bytes) {

@@ -72,7 +72,7 @@ def float32_coefficients(degree: int = 3) -> tuple[list[float], float]:
 
 
 def main() -> int:
-    for degree in (3, 4):
+    for degree in (3, 4, 5):
         coeffs, bound = float32_coefficients(degree)
         print(f"degree {degree}: relative error bound {bound:.3e}")
         for i, c in enumerate(coeffs):

@@ -433,6 +433,31 @@ __device__ __forceinline__ void exp2_poly_x2(uint64_t x2, float& r0, float& r1) 
   r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
+// The same with the polynomial of degree 5 (relative error < 2.2e-7, evaluated in fp32).
+__device__ __forceinline__ void exp2_poly5_x2(uint64_t x2, float& r0, float& r1) {
+  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
+  const uint64_t neg_magic = f2_pack(-12582912.0f, -12582912.0f);
+  const uint64_t minus_one = f2_pack(-1.0f, -1.0f);
+  const uint64_t d5 = f2_pack(0.0013276472454890609f, 0.0013276472454890609f);
+  const uint64_t d4 = f2_pack(0.009675540961325169f, 0.009675540961325169f);
+  const uint64_t d3 = f2_pack(0.05550713092088699f, 0.05550713092088699f);
+  const uint64_t d2 = f2_pack(0.24022120237350464f, 0.24022120237350464f);
+  const uint64_t d1 = f2_pack(0.6931469440460205f, 0.6931469440460205f);
+  const uint64_t d0 = f2_pack(1.0000001192092896f, 1.0000001192092896f);
+  const uint64_t t2 = f2_add(x2, magic);
+  const uint64_t f2 = f2_fma(f2_add(t2, neg_magic), minus_one, x2);
+  uint64_t p2 = f2_fma(d5, f2, d4);
+  p2 = f2_fma(p2, f2, d3);
+  p2 = f2_fma(p2, f2, d2);
+  p2 = f2_fma(p2, f2, d1);
+  p2 = f2_fma(p2, f2, d0);
+  float p0, p1, t0, t1;
+  f2_unpack(p2, p0, p1);
+  f2_unpack(t2, t0, t1);
+  r0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
 // Packs two floats to bf16x2 with round-to-nearest-even: `lo` in bits 0-15.
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   uint32_t r;

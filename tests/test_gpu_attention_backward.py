@@ -160,14 +160,42 @@ def test_grouped_forward_matches_fp64(b200, training, case):
     assert float((got_lse.double() - lse)[~empty].abs().max()) <= 1e-3
 
 
-def test_equal_shapes_give_the_candidate_forwards_bits(b200, training):
+def test_equal_shapes_agree_with_the_candidate_forward(b200, training):
+    # The same kernel but for the polynomial of its exponentials (relative errors 2.2e-7 and
+    # 7.5e-5): both round P and the output to bf16, the LSEs differ by the larger error.
     import torch
 
     for case in [(1, 4, 4, 512, 512, False), (1, 4, 4, 500, 500, True)]:
-        q, k, v, _ = make(case, seed=3)
+        q, k, v, do = make(case, seed=3)
+        exact, lse64, _, _ = plain(q, k, v, do, case[5], b200.default_scale())
         out, lse = training.grouped_attention(q, k, v, case[5])
         want, want_lse = b200.attention_forward(q, k, v, case[5])
-        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        s = q.double() @ k.double().transpose(-1, -2) * b200.default_scale()
+        p = torch.exp(s - lse64[..., None])
+        if case[5]:
+            p = p.tril()
+        bound = 2 * (U + 1.5e-4) * (p @ v.double().abs()) + 2 * U * exact.abs()
+        assert bool(((out.double() - want.double()).abs() <= bound).all())
+        assert float((lse - want_lse).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("seq", [1, 4, 64, 300, 1000])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lse_has_fp32_precision(b200, training, seq, causal):
+    # Inputs of a few bits: the scores are exact.  What is left: 2.5e-7 of every exponential,
+    # one step per addition of the row sum, and a few of the terms of LSE = m + log(sum).
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(seq)
+    q, k, v = (torch.randint(-2, 3, (2, 4, seq, 128), device="cuda", generator=gen).bfloat16() / 2 for _ in range(3))
+    out, lse = training.grouped_attention(q, k, v, causal)
+    s = q.double() @ k.double().transpose(-1, -2) * b200.default_scale()
+    if causal:
+        s = s.masked_fill(torch.ones((seq, seq), device="cuda", dtype=torch.bool).triu(1), -math.inf)
+    want = torch.logsumexp(s, -1)
+    most = s.masked_fill(s == -math.inf, 0).abs().amax(-1)
+    bound = 2.5e-7 + seq * EPS32 + 8 * EPS32 * (want.abs() + most)
+    assert bool(((lse.double() - want).abs() <= bound).all())
 
 
 def test_rows_without_keys_get_zero_gradients(b200, training):

@@ -122,3 +122,25 @@ def test_python_checks_without_a_gpu():
         seed.qkv_norm_rope(q, 2, 3, lse, lse)
     with pytest.raises(RuntimeError, match="dq must be a CUDA tensor"):
         seed.qkv_norm_rope_backward(q, q, q, q, lse, lse)
+
+
+def test_degree_five_exponential_is_the_fitted_polynomial():
+    """The constants of exp2_poly5_x2 are what exp2_poly.py derives, within the stated error."""
+    import importlib.util
+    import re
+    from pathlib import Path
+
+    import numpy as np
+
+    here = Path(__file__).resolve().parents[1] / "avo-ampere_b200" / "candidates" / "cuda_b200_attention"
+    spec = importlib.util.spec_from_file_location("avo_b200_exp2_fit_5", here / "exp2_poly.py")
+    fit = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(fit)
+    found = dict(re.findall(r"d(\d) = f2_pack\(([-0-9.e]+)f,", (here / "sm100_ptx.cuh").read_text()))
+    header = np.float32([float(found[str(i)]) for i in range(6)])
+    assert np.array_equal(header, np.float32(fit.float32_coefficients(5)[0]))
+    f = np.linspace(-0.5, 0.5, 400_001).astype(np.float32)
+    p = np.full_like(f, header[5])
+    for c in header[4::-1]:
+        p = (p.astype(np.float64) * f + c).astype(np.float32)  # an fp32 FMA
+    assert np.abs(p / np.exp2(f.astype(np.float64)) - 1).max() < 2.2e-7
