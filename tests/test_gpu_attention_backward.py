@@ -468,3 +468,26 @@ def test_empty_sizes(b200, training):
         assert bool((out == 0).all()) and bool((lse == -math.inf).all())
         for g, like in zip(grads, (q, k, v)):
             assert g.shape == like.shape and bool((g == 0).all())
+
+
+def test_offsets_past_32_bits(b200, training):
+    # q, out and their gradients have more than 2^31 elements; the last heads against the formula.
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 60 GB of device memory")
+    case = (16, 1024, 256, 1100, 1100, True)
+    q, k, v, do = make(case, seed=21)
+    assert q.numel() > 2**31
+    out, lse = training.grouped_attention(q, k, v, True)
+    heads, kv_heads = slice(-8, None), slice(-2, None)
+    sq, sk, sv, sdo = (t[-1:, h].contiguous() for t, h in ((q, heads), (k, kv_heads), (v, kv_heads), (do, heads)))
+    exact, lse64, want, bounds = plain(sq, sk, sv, sdo, True, b200.default_scale())
+    assert float((out[-1:, heads].double() - exact).abs().max()) <= 2e-2
+    assert float((lse[-1:, heads].double() - lse64).abs().max()) <= 1e-3
+    out[-1:, heads] = exact.bfloat16()
+    lse[-1:, heads] = lse64.float()
+    grads = training.attention_backward(do, q, k, v, out, lse, True)
+    torch.cuda.synchronize()
+    for name, g, h, w, bound in zip(("dq", "dk", "dv"), grads, (heads, kv_heads, kv_heads), want, bounds):
+        assert_within(g[-1:, h], w, bound, name)

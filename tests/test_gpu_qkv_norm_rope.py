@@ -412,3 +412,34 @@ def test_empty_sizes(b200, seed):
         assert q.shape == (batch, 2, seq, 128) and k.shape == v.shape == (batch, 1, seq, 128)
         dqkv, dqw, dkw = seed.qkv_norm_rope_backward(*grads, qkv, cos, sin, **how)
         assert dqkv.shape == qkv.shape and bool((dqw == 0).all()) and bool((dkw == 0).all())
+
+
+def test_offsets_past_32_bits(b200, seed):
+    # A projection of more than 2^31 elements: its last tokens equal a call on them alone.
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of device memory")
+    gen = torch.Generator(device="cuda").manual_seed(5)
+
+    def randn(*shape):
+        return torch.randn(shape, device="cuda", generator=gen, dtype=torch.bfloat16)
+
+    batch, seq, heads, kv_heads, last = 2, 351_001, 16, 4, 70
+    qkv = randn(batch, seq, heads + 2 * kv_heads, 128)
+    assert qkv.numel() > 2**31
+    angle = torch.rand((1000, 64), device="cuda", generator=gen) * 6
+    cos, sin = angle.cos(), angle.sin()
+    positions = torch.arange(seq, device="cuda") % 1000
+    w = 1 + torch.rand(128, device="cuda", generator=gen)
+    how = dict(q_weight=w, k_weight=w)
+    outs = seed.qkv_norm_rope(qkv, heads, kv_heads, cos, sin, positions=positions, **how)
+    tail = seed.qkv_norm_rope(qkv[-1:, -last:], heads, kv_heads, cos, sin, positions=positions[-last:], **how)
+    for got, want in zip(outs, tail):
+        assert torch.equal(got[-1:, :, -last:], want)
+    grads = [randn(*t.shape) for t in outs]
+    del outs
+    dqkv, _, _ = seed.qkv_norm_rope_backward(*grads, qkv, cos, sin, positions=positions, **how)
+    few = [g[-1:, :, -last:].contiguous() for g in grads]
+    want, _, _ = seed.qkv_norm_rope_backward(*few, qkv[-1:, -last:], cos, sin, positions=positions[-last:], **how)
+    assert torch.equal(dqkv[-1:, -last:], want)
