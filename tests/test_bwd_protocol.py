@@ -1,7 +1,7 @@
 """A model of the attention-gradient kernel's synchronisation protocol, run on the CPU.
 
-attn_bwd.cuh runs, per CTA, a producer, a waiter, an MMA issuer, eight softmax warps and an
-epilogue warpgroup over the flat sequence of its items' tiles, in two variants (dK/dV and
+attn_bwd.cuh runs, per CTA, a producer, a waiter, an MMA issuer, four softmax warpgroups (two
+in this model) and an epilogue warpgroup over the flat sequence of its items' tiles, in two variants (dK/dV and
 dQ).  As for the forward kernel, each role's schedule is restated as a generator and run
 under random interleavings with asynchronous copies and an in-order tensor pipe; the model
 checks that every schedule ends, that no named barrier keeps arrivals, and that no buffer
