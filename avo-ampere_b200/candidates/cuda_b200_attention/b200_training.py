@@ -12,7 +12,8 @@ current CUDA stream of the tensors' device, the device's status word, no fallbac
 * ``qkv_norm_rope_backward``: its gradient as a plain call.
 
 Scratch is allocated per call by torch's caching allocator on the current stream, so calls
-on several streams, and several captured graphs, share nothing but the status word.
+on several streams, and several captured graphs, share nothing but the status word.  The plain
+calls can be captured in a CUDA graph, after one call on the device (which creates that word).
 """
 
 from __future__ import annotations
