@@ -141,12 +141,13 @@ def _forward(q, k, v, causal: bool, scale: float):
     b.load_library()
     index = q.get_device()
     with _on(index):
-        size = _forward_scratch_bytes(index)
-        scratch = q.new_empty(size, dtype=torch.uint8)
+        # Only unmasked work (a single query's is) is split between CTAs.
+        size = _forward_scratch_bytes(index) if not causal or seq_q == 1 else 0
+        scratch = q.new_empty(size, dtype=torch.uint8) if size else None
         code = b.call_entry(
             0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,
-            seq_kv, HEAD_DIM, 1 if causal else 0, scale, scratch.data_ptr(), size, b.status_address(index),
-            b._raw_stream(index))
+            seq_kv, HEAD_DIM, 1 if causal else 0, scale, None if scratch is None else scratch.data_ptr(), size,
+            b.status_address(index), b._raw_stream(index))
     b._check(code, "avo_b200_attn_fwd_grouped")
     return out, lse
 
