@@ -296,9 +296,10 @@ int g_plans_next = 0;
 // Returns a copy (this thread's own) of the cached entry: another thread may replace the
 // cache slot as soon as the lock is released.
 const PlanEntry& cached_plan(int num_bh, int seq_q, int seq_kv, int causal, long long q_pos0, long long kv_pos0,
-                             int sms, bool split_ok) {
+                             int sms, bool split_ok, bool lists_ok) {
   static thread_local PlanEntry mine;
-  const long long key[8] = {num_bh, seq_q, seq_kv, causal ? 1 : 0, q_pos0, kv_pos0, sms, split_ok ? 1 : 0};
+  const long long key[8] = {num_bh, seq_q, seq_kv, causal ? 1 : 0, q_pos0, kv_pos0, sms,
+                            (split_ok ? 1 : 0) + (lists_ok ? 2 : 0)};
   std::lock_guard<std::mutex> lock(g_mu);
   for (int e = 0; e < g_plans_used; ++e) {
     bool same = true;
@@ -314,16 +315,22 @@ const PlanEntry& cached_plan(int num_bh, int seq_q, int seq_kv, int causal, long
   g_plans_next = (g_plans_next + 1) % kPlanCache;
   if (g_plans_used < kPlanCache) ++g_plans_used;
   for (int i = 0; i < 8; ++i) entry.key[i] = key[i];
-  entry.plan = sched::make_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sms, split_ok, &entry.table.t);
+  entry.plan =
+      sched::make_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sms, split_ok, lists_ok, &entry.table.t);
   mine = entry;
   return mine;
 }
 
+// `grouped`: what avo_b200_attn_fwd_grouped runs.  Its LSE is saved for a gradient, so it takes
+// the kernels whose LSE has fp32 precision, and causal work takes the list plan with or without a
+// workspace (the other entries need one for it: without it they promise waves).  Measured on
+// B200, causal, waves / lists: B2 H16 Hkv4 S4096 148.9 / 142.5 us, B2 H16 S8192 545 / 525, B8 H16
+// S2048 193.5 / 179.9, B4 H32 Hkv8 S4096 592 / 555.
 int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int num_bh,
                int seq_q, int seq_kv, int head_dim, long long q_hs, long long kv_hs, long long o_hs,
                long long lse_hs, int causal, float scale, long long q_pos0, long long kv_pos0,
                int* status, void* stream, void* workspace = nullptr, size_t workspace_bytes = 0, int kv_group = 1,
-               bool fine = false) {
+               bool grouped = false) {
   if (q == nullptr || k == nullptr || v == nullptr || o == nullptr) return AVO_B200_EINVAL;
   if (head_dim != kHeadDim || num_bh < 0 || seq_q < 0 || seq_kv < 0) return AVO_B200_EINVAL;
   if (!(scale > 0.f) || !std::isfinite(scale)) return AVO_B200_EINVAL;
@@ -350,7 +357,8 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
   const bool split_ok = workspace != nullptr && cooperative_ok();
   if (workspace != nullptr && workspace_bytes < workspace_bytes_for(sm_count)) return AVO_B200_EINVAL;
   if (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return AVO_B200_EINVAL;
-  const PlanEntry& entry = cached_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sm_count, split_ok);
+  const PlanEntry& entry =
+      cached_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sm_count, split_ok, split_ok || grouped);
   const sched::Plan plan = entry.plan;
   const int grid = plan.grid;
 
@@ -386,6 +394,7 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
   p.scale_log2 = scale * 1.4426950408889634f;
 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto* const plain_kernel = grouped ? attn_fwd_kernel<false, 5> : attn_fwd_kernel<false, 3>;
   if (plan.mode == sched::kWaves) {
     // Programmatic dependent launch: this launch's CTAs may start their set-up on free
     // multiprocessors while the previous work in the stream finishes (the kernel waits for
@@ -403,12 +412,12 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, fine ? attn_fwd_kernel<false, 5> : attn_fwd_kernel<false, 3>, tm_q, tm_k, tm_v, p, TableParam<false>{0}) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, plain_kernel, tm_q, tm_k, tm_v, p, TableParam<false>{0}) != cudaSuccess) {
       (void)cudaGetLastError();
       return AVO_B200_ELAUNCH;
     }
   } else if (plan.mode == sched::kTable) {
-    auto* kernel = fine ? attn_fwd_kernel<true, 5> : attn_fwd_kernel<true, 3>;
+    auto* kernel = grouped ? attn_fwd_kernel<true, 5> : attn_fwd_kernel<true, 3>;
     kernel<<<static_cast<unsigned>(grid), kThreads, kSmemBytes, st>>>(tm_q, tm_k, tm_v, p, entry.table);
   } else {
     // Split pieces: a CTA that merges an item waits for its neighbours' continuation
@@ -416,14 +425,39 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
     // (or fails to launch).
     TableParam<false> none{0};
     void* args[] = {&tm_q, &tm_k, &tm_v, &p, &none};
-    if (cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(fine ? attn_fwd_kernel<false, 5> : attn_fwd_kernel<false, 3>), dim3(grid),
-                                    dim3(kThreads), args, kSmemBytes, st) != cudaSuccess) {
+    if (cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(plain_kernel), dim3(grid), dim3(kThreads), args,
+                                    kSmemBytes, st) != cudaSuccess) {
       (void)cudaGetLastError();
       return AVO_B200_ELAUNCH;
     }
   }
   if (cudaGetLastError() != cudaSuccess) return AVO_B200_ELAUNCH;
   return AVO_B200_OK;
+}
+
+// What avo_b200_attn_fwd_grouped launches for its sizes.
+struct Grouped {
+  int pairs;         // heads of the launch, over the batch
+  int seq_q, group;  // rows per head; heads per key/value head
+  int causal;
+  long long q_pos0;  // position of the first query
+};
+bool grouped_launch(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal, Grouped* g) {
+  if (batch < 0 || heads < 0 || kv_heads <= 0 || seq_q < 0 || seq_kv < 0 || heads % kv_heads != 0) return false;
+  const long long bh = static_cast<long long>(batch) * heads;
+  if (bh > INT_MAX) return false;
+  *g = {static_cast<int>(bh), seq_q, heads / kv_heads, causal, 0};
+  if (seq_q == 1 && seq_kv > 0) g->causal = 0;  // a single query sees every key
+  if (!g->causal && g->group > 1 && static_cast<long long>(g->group) * seq_q <= INT_MAX / 2) {
+    // Without a mask the rows of the heads that share a key/value head attend alike, and they
+    // are adjacent in memory: one head of group * seq_q rows, whose keys are read once.
+    g->seq_q = seq_q * g->group;
+    g->pairs = batch * kv_heads;
+    g->group = 1;
+  }
+  // With a mask, query row i sits at position seq_kv - seq_q + i: the last query sees every key.
+  if (g->causal) g->q_pos0 = static_cast<long long>(seq_kv) - seq_q;
+  return true;
 }
 
 }  // namespace
@@ -474,41 +508,45 @@ extern "C" int avo_b200_attn_fwd_grouped(const void* q, const void* k, const voi
                                          int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
                                          float softmax_scale, void* workspace, size_t workspace_bytes,
                                          int* status_dev, void* stream) {
-  if (batch < 0 || heads < 0 || kv_heads <= 0 || seq_q < 0 || seq_kv < 0 || heads % kv_heads != 0)
-    return AVO_B200_EINVAL;
-  const long long bh = static_cast<long long>(batch) * heads;
-  if (bh > INT_MAX) return AVO_B200_EINVAL;
-  int group = heads / kv_heads;
-  long long pairs = bh;
-  if (seq_q == 1 && seq_kv > 0) causal = 0;  // a single query sees every key
-  if (!causal && group > 1 && static_cast<long long>(group) * seq_q <= INT_MAX / 2) {
-    // Without a mask the rows of the heads that share a key/value head attend alike, and they
-    // are adjacent in memory: one head of group * seq_q rows, whose keys are read once.
-    seq_q *= group;
-    pairs = static_cast<long long>(batch) * kv_heads;
-    group = 1;
-  }
-  const long long qhs = static_cast<long long>(seq_q) * kHeadDim, khs = static_cast<long long>(seq_kv) * kHeadDim;
-  if (workspace != nullptr && bh > 0 && seq_q > 0 && head_dim == kHeadDim) {
+  Grouped g;
+  if (!grouped_launch(batch, heads, kv_heads, seq_q, seq_kv, causal, &g)) return AVO_B200_EINVAL;
+  const long long qhs = static_cast<long long>(g.seq_q) * kHeadDim, khs = static_cast<long long>(seq_kv) * kHeadDim;
+  if (workspace != nullptr && g.pairs > 0 && seq_q > 0 && head_dim == kHeadDim) {
     // Only the split plan uses the workspace; its flags (at the front) have to start at zero.
     if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return AVO_B200_EINVAL;
     int sms = 0;
     const int rc = prepare_device(&sms);
     if (rc != AVO_B200_OK) return rc;
     if (workspace_bytes < workspace_bytes_for(sms)) return AVO_B200_EINVAL;
-    const long long items = pairs * ((static_cast<long long>(seq_q) + kRowsPerCta - 1) / kRowsPerCta);
-    if (items <= INT_MAX && !causal && cooperative_ok() &&
-        cached_plan(static_cast<int>(pairs), seq_q, seq_kv, 0, 0, 0, sms, true).plan.mode == sched::kTail &&
+    const long long items = g.pairs * ((static_cast<long long>(g.seq_q) + kRowsPerCta - 1) / kRowsPerCta);
+    if (items <= INT_MAX && !g.causal && cooperative_ok() &&
+        cached_plan(g.pairs, g.seq_q, seq_kv, 0, 0, 0, sms, true, true).plan.mode == sched::kTail &&
         cudaMemsetAsync(workspace, 0, static_cast<size_t>(sms) * kFlagBytesPerCta, static_cast<cudaStream_t>(stream)) !=
             cudaSuccess) {
       (void)cudaGetLastError();
       return AVO_B200_ELAUNCH;
     }
   }
-  // With a mask, query row i sits at position seq_kv - seq_q + i: the last query sees every key.
-  return launch_fwd(q, k, v, o, lse, static_cast<int>(pairs), seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim,
-                    qhs, seq_q, causal, softmax_scale, causal ? static_cast<long long>(seq_kv) - seq_q : 0, 0,
-                    status_dev, stream, workspace, workspace_bytes, group, true);
+  return launch_fwd(q, k, v, o, lse, g.pairs, g.seq_q, seq_kv, head_dim, qhs, khs > 0 ? khs : kHeadDim, qhs, g.seq_q,
+                    g.causal, softmax_scale, g.q_pos0, 0, status_dev, stream, workspace, workspace_bytes, g.group, true);
+}
+
+extern "C" int avo_b200_attn_fwd_grouped_plan(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal,
+                                              int sm_count, int split, int* plan_out) {
+  Grouped g;
+  if (sm_count <= 0 || plan_out == nullptr || !grouped_launch(batch, heads, kv_heads, seq_q, seq_kv, causal, &g))
+    return AVO_B200_EINVAL;
+  const long long blocks = (static_cast<long long>(g.seq_q) + kRowsPerCta - 1) / kRowsPerCta;
+  const long long kv_tiles = (static_cast<long long>(seq_kv) + kBlockN - 1) / kBlockN;
+  if (g.pairs * blocks > INT_MAX || (kv_tiles > 0 && g.pairs * blocks > INT_MAX / kv_tiles)) return AVO_B200_EINVAL;
+  static thread_local sched::Table table;
+  const sched::Plan plan = sched::make_plan(g.pairs, g.seq_q, seq_kv, g.causal, g.q_pos0, 0, sm_count, split != 0,
+                                            true, &table);
+  plan_out[0] = plan.mode;
+  plan_out[1] = plan.grid;
+  plan_out[2] = plan.mode == sched::kTable ? plan.group_pairs : plan.run_min;
+  plan_out[3] = plan.wave_items;
+  return AVO_B200_OK;
 }
 
 extern "C" int avo_b200_attn_workspace_size(size_t* bytes) {
@@ -538,7 +576,7 @@ extern "C" int avo_b200_schedule_units(int num_bh, int seq_q, int seq_kv, int ca
     return AVO_B200_EINVAL;
   static thread_local sched::Table table;
   const sched::Plan plan =
-      sched::make_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sm_count, split != 0, &table);
+      sched::make_plan(num_bh, seq_q, seq_kv, causal, q_pos0, kv_pos0, sm_count, split != 0, split != 0, &table);
   plan_out[0] = plan.mode;
   plan_out[1] = plan.grid;
   plan_out[2] = plan.mode == sched::kTable ? plan.group_pairs : plan.run_min;

@@ -64,6 +64,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, ctypes.c_size_t,
          _vp, _vp],
     ),
+    "avo_b200_attn_fwd_grouped_plan": (_c_int, [_c_int] * 8 + [_vp]),
     "avo_b200_attn_bwd_workspace_size": (
         _c_int,
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
@@ -526,3 +527,14 @@ def schedule_units(num_bh: int, seq_q: int, seq_kv: int, causal: bool, *, sm_cou
     if (counts > max_units).any():
         raise ValueError(f"more than {max_units} units per CTA")
     return plan[0], grid, plan[2], plan[3], [units[c, :counts[c]].tolist() for c in range(grid)]
+
+
+def grouped_plan(batch: int, heads: int, kv_heads: int, seq_q: int, seq_kv: int, causal: bool, *, sm_count: int = 148,
+                 split: bool = True) -> tuple[int, int, int, int]:
+    """(mode, grid, run_min, wave_items) of the plan that the grouped forward runs for these sizes, with or
+    without a workspace (``split``); needs no GPU.  Modes as in schedule_units."""
+    plan = (ctypes.c_int * 4)()
+    code = load_library().avo_b200_attn_fwd_grouped_plan(batch, heads, kv_heads, seq_q, seq_kv, 1 if causal else 0,
+                                                         sm_count, 1 if split else 0, plan)
+    _check(code, "avo_b200_attn_fwd_grouped_plan")
+    return tuple(plan)

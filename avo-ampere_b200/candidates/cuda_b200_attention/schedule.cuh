@@ -171,9 +171,6 @@ __host__ __device__ inline void locate(const Plan& p, const Segment& g, int pos,
   n = p.n_kv;
 }
 
-// Chooses the plan of a launch.  `split_ok`: the caller provided scratch for split pieces
-// and the launch can hold all CTAs resident at once (a cooperative launch); without it
-// every item stays whole (kWaves).  `sms`: multiprocessors, one CTA each.
 // kTable's lists for group size g: greedy list scheduling of the grouped order, each
 // item's cost its tile count plus one tile of fixed per-item work.  Returns the largest
 // CTA load; fills `t` if non-null.
@@ -230,8 +227,12 @@ inline long long build_table(const Plan& p, int g, Table* t) {
   return worst;
 }
 
+// Chooses the plan of a launch.  `split_ok`: the caller provided scratch for split pieces
+// and the launch can hold all CTAs resident at once (a cooperative launch); without it
+// every item stays whole.  `lists_ok`: causal work may take kTable's lists (whole items,
+// which need no scratch), written to `table`.  `sms`: multiprocessors, one CTA each.
 inline Plan make_plan(int num_bh, int seq_q, int seq_kv, int causal, long long q_pos0, long long kv_pos0, int sms,
-                      bool split_ok, Table* table = nullptr) {
+                      bool split_ok, bool lists_ok, Table* table) {
   Plan p{};
   p.mode = kWaves;
   p.num_bh = num_bh;
@@ -244,9 +245,10 @@ inline Plan make_plan(int num_bh, int seq_q, int seq_kv, int causal, long long q
   const long long items = static_cast<long long>(num_bh) * p.nq;
   p.grid = static_cast<int>(items < sms ? items : sms);
   p.run_min = 1;
-  if (!split_ok || items == 0 || p.n_kv == 0 || sms <= 1) return p;
+  if (items == 0 || p.n_kv == 0 || sms <= 1) return p;
   const int run_min = (p.n_kv + 3) / 4 > 4 ? (p.n_kv + 3) / 4 : 4;
-  if (!p.causal && static_cast<long long>(items) * p.n_kv <= 0x7fffffffll) {
+  if (!p.causal) {
+    if (!split_ok || items * p.n_kv > 0x7fffffffll) return p;
     // Whole items: F full waves and a last wave of R items, (F + 1) * T tiles per CTA at
     // most.  Split: the R tail items' tiles spread evenly.  Take the split when it saves
     // at least 3 % (a split piece costs about two tiles of extra epilogue work).
@@ -263,15 +265,14 @@ inline Plan make_plan(int num_bh, int seq_q, int seq_kv, int causal, long long q
     p.grid = F > 0 ? sms : static_cast<int>((R * T + run - 1) / run);
     return p;
   }
-  // Causal: whole items.  With a workspace (split_ok, checked above: launches without one
-  // keep the longest-first waves), room for kTable's lists and at least two items per SM,
-  // the grouped greedy plan: the smallest group whose pairs' K/V fit in 48 MB among those
+  // Causal: whole items.  Where the launch may take lists, with room for them and at least
+  // two items per SM, the grouped greedy plan: the smallest group whose pairs' K/V fit in 48 MB among those
   // within 2 % of the best makespan over all group sizes; otherwise longest first over all
   // heads in waves (within ~2 % of the mean tile count per CTA on the causal workloads).
   // Head-grouped stream-K plans for causal work were measured on B200 and ran 20-27 %
   // slower: runs over a pair's first q blocks hold many 2-6 tile units, whose fixed
   // per-unit costs the tile balance does not see.
-  if (table == nullptr || items < 2ll * sms || items > kTableItems || sms > kTableCtas) return p;
+  if (!lists_ok || items < 2ll * sms || items > kTableItems || sms > kTableCtas) return p;
   const long long pair_kv = static_cast<long long>(seq_kv) * 128 * 2 * 2;
   const int candidates[] = {num_bh, 32, 24, 16, 12, 8, 6, 4, 3, 2, 1};
   long long best = -1;

@@ -182,13 +182,22 @@ int avo_b200_attn_fwd_split_noalloc(const void* q, const void* k, const void* v,
  * ends: query i sees keys j <= i + seq_kv - seq_q, so with seq_q > seq_kv the first
  * queries see none (o = 0, lse = -inf).  workspace: null (whole work items only), or
  * device memory of avo_b200_attn_workspace_size() bytes, 256-byte aligned, uninitialised,
- * which lets the kernel cut items between CTAs as avo_b200_attn_fwd_ws does; calls that may
- * overlap in time need a workspace each.  No reference counterpart.
+ * which lets the kernel cut items of unmasked work between CTAs as avo_b200_attn_fwd_ws does;
+ * calls that may overlap in time need a workspace each.  Causal work is never cut and takes
+ * the plan of lists (mode 2) with or without a workspace.  No reference counterpart.
  */
 int avo_b200_attn_fwd_grouped(const void* q, const void* k, const void* v, void* o, float* lse, int batch,
                               int heads, int kv_heads, int seq_q, int seq_kv, int head_dim, int causal,
                               float softmax_scale, void* workspace, size_t workspace_bytes,
                               int* status_dev, void* stream);
+
+/*
+ * Diagnostic (host only, needs no GPU): the plan that avo_b200_attn_fwd_grouped runs for these
+ * sizes on `sm_count` multiprocessors, with (split != 0) or without a workspace.  plan_out as
+ * in avo_b200_schedule_units; a workspace is only used in mode 1.
+ */
+int avo_b200_attn_fwd_grouped_plan(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal,
+                                   int sm_count, int split, int* plan_out);
 
 /*
  * Gradient of avo_b200_attn_fwd_grouped (and, with kv_heads == heads and seq_kv == seq_q,

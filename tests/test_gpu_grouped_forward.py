@@ -1,0 +1,103 @@
+"""grouped_attention on a B200 against 64 bits, with the bounds that its formulas give and no slack.
+
+With u = 2^-8 (half a bf16 step), eps = 2^-24, A = scale * sum_d |q k| and M = max_j |s| of a row,
+a probability's fp32 value before the division by the row sum has the relative error
+
+    e_j = 2.5e-7 (the exponential) + 128 eps A_j (the dot product) + 3 eps |s_j| (the scale's
+          roundings) + eps (|s_j| + M + 11) (the exponent: the row's reference value lies within
+          2^15, that is 10.4 in natural units, of its maximum)
+
+and joining the pieces of a row multiplies by at most eight exponentials, e_m = 8 (2.5e-7 +
+eps (2 M + 11)).  The row sum l adds n keys: its relative error is L = sum_j P_j e_j + n eps + e_m.
+P is rounded to bf16 for the product with V, whose n terms are added in fp32; the output is
+divided by l (two roundings) and rounded once:
+
+    |O err|   <= 1.01 (sum_j P_j |V_j| (u + e_j + e_m + n eps) + |O| (L + 2 eps)) + u |O|
+    |LSE err| <= L + 8 eps (|LSE| + M + 1)
+
+where 1.01 covers the products of two of these errors.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+from test_gpu_attention_backward import CASES, EPS32, U, make
+
+pytestmark = pytest.mark.gpu
+
+# Causal, from two items of 256 rows per multiprocessor on: whole items in lists, several query
+# heads to a key/value head among them.
+LISTS = [
+    # batch, heads, kv_heads, seq_q, seq_kv, causal
+    (2, 16, 4, 2400, 2400, True),
+    (4, 32, 8, 1111, 1500, True),
+    (2, 96, 1, 513, 300, True),      # rows that see no key, one key/value head for all
+    (37, 8, 2, 129, 700, True),
+    (1, 512, 128, 1025, 1025, True),
+]
+
+
+@pytest.fixture(scope="module")
+def seed():
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "avo-ampere_b200" / "candidates" / "cuda_b200_attention_seed.py"
+    spec = importlib.util.spec_from_file_location("avo_candidate_b200_seed_grouped", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def check(b200, q, k, v, causal, got, got_lse):
+    """Compares out and lse with the formula, one batch entry and key/value head at a time."""
+    import torch
+
+    scale = b200.default_scale()
+    batch, heads, seq_q, _ = q.shape
+    kv_heads, n = k.shape[1], k.shape[2]
+    group = heads // kv_heads
+    hidden = torch.arange(n, device=q.device) > torch.arange(seq_q, device=q.device)[:, None] + n - seq_q
+    for b in range(batch):
+        for g in range(kv_heads):
+            mine = slice(g * group, (g + 1) * group)
+            qh, kh, vh = q[b, mine].double(), k[b, g].double(), v[b, g].double()
+            s = scale * (qh @ kh.T)
+            if causal:
+                s = s.masked_fill(hidden, -math.inf)
+            lse = torch.logsumexp(s, -1)
+            empty = lse == -math.inf
+            p = torch.exp(s - torch.where(empty, 0.0, lse)[..., None])
+            out = p @ vh
+            size = s.abs().masked_fill(s == -math.inf, 0.0)
+            most = size.amax(-1) if n else torch.zeros_like(lse)
+            e = 2.5e-7 + 128 * EPS32 * scale * (qh.abs() @ kh.abs().T) + EPS32 * (4 * size + most[..., None] + 11)
+            e_m = 8 * (2.5e-7 + EPS32 * (2 * most + 11))
+            total = (p * e).sum(-1) + n * EPS32 + e_m
+            bound = 1.01 * ((p * (U + e + e_m[..., None] + n * EPS32)) @ vh.abs()
+                            + out.abs() * (total[..., None] + 2 * EPS32)) + U * out.abs()
+            err = (got[b, mine].double() - out).abs()
+            assert bool((err <= bound + 1e-30).all()), ("out", b, g, float((err / (bound + 1e-30)).max()))
+            mine_lse = got_lse[b, mine]
+            assert torch.equal(mine_lse == -math.inf, empty) and bool((got[b, mine][empty] == 0).all())
+            err = (mine_lse.double() - lse).abs()[~empty]
+            allowed = (total + 8 * EPS32 * (lse.abs() + most + 1))[~empty]
+            assert bool((err <= allowed).all()), ("lse", b, g, float((err / allowed).max()))
+
+
+@pytest.mark.parametrize("case", CASES + LISTS)
+def test_forward_within_the_derived_bounds(b200, seed, case):
+    import torch
+
+    q, k, v, _ = make(case, seed=31)
+    if case in LISTS:
+        assert b200.grouped_plan(*case, sm_count=torch.cuda.get_device_properties(0).multi_processor_count,
+                                 split=False)[0] == 2
+    got, got_lse = seed.grouped_attention(q, k, v, case[5])
+    again, again_lse = seed.grouped_attention(q, k, v, case[5])
+    torch.cuda.synchronize()
+    b200.check_status(q.device)
+    assert torch.equal(got, again) and torch.equal(got_lse, again_lse)
+    check(b200, q, k, v, case[5], got, got_lse)
