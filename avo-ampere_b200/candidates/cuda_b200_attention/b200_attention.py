@@ -90,6 +90,7 @@ STATUS_WATCHDOG = 1
 STATUS_DRAIN = 2
 STATUS_POSITION = 4
 NOALLOC_MAX_ROWS = 16384  # AVO_B200_NOALLOC_MAX_ROWS
+PLAN_SPLIT = 1  # mode of a plan that cuts items between CTAs (schedule_units, grouped_plan)
 ETOOBIG = 6
 EREGS = 7
 

@@ -117,16 +117,19 @@ def _scale(softmax_scale) -> float:
     return scale
 
 
-_forward_scratch: dict[int, int] = {}
-
-
-def _forward_scratch_bytes(index: int) -> int:
-    """Scratch of the forward's split plan on device ``index`` (a function of the device alone)."""
-    if index not in _forward_scratch:
-        size = ctypes.c_size_t(0)
-        b._check(b.load_library().avo_b200_attn_workspace_size(ctypes.byref(size)), "avo_b200_attn_workspace_size")
-        _forward_scratch[index] = size.value
-    return _forward_scratch[index]
+@functools.lru_cache(maxsize=256)
+def _forward_scratch_bytes(index: int, batch: int, heads: int, kv_heads: int, seq_q: int, seq_kv: int,
+                           causal: bool) -> int:
+    """Scratch of the forward for these sizes on device ``index``, the current one: what a plan that
+    splits items between CTAs needs, 0 for the others (causal work is never split)."""
+    if causal and seq_q > 1:
+        return 0
+    sms = _torch().cuda.get_device_properties(index).multi_processor_count
+    if b.grouped_plan(batch, heads, kv_heads, seq_q, seq_kv, causal, sm_count=sms)[0] != b.PLAN_SPLIT:
+        return 0
+    size = ctypes.c_size_t(0)
+    b._check(b.load_library().avo_b200_attn_workspace_size(ctypes.byref(size)), "avo_b200_attn_workspace_size")
+    return size.value
 
 
 def _forward(q, k, v, causal: bool, scale: float):
@@ -141,8 +144,7 @@ def _forward(q, k, v, causal: bool, scale: float):
     b.load_library()
     index = q.get_device()
     with _on(index):
-        # Only unmasked work (a single query's is) is split between CTAs.
-        size = _forward_scratch_bytes(index) if not causal or seq_q == 1 else 0
+        size = _forward_scratch_bytes(index, batch, heads, kv_heads, seq_q, seq_kv, bool(causal))
         scratch = q.new_empty(size, dtype=torch.uint8) if size else None
         code = b.call_entry(
             0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, heads, kv_heads, seq_q,

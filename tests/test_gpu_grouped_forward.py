@@ -101,3 +101,24 @@ def test_forward_within_the_derived_bounds(b200, seed, case):
     b200.check_status(q.device)
     assert torch.equal(got, again) and torch.equal(got_lse, again_lse)
     check(b200, q, k, v, case[5], got, got_lse)
+
+
+@pytest.mark.parametrize("case,splits", [((1, 4, 1, 512, 512, True), False), ((4, 16, 16, 1184, 256, False), False),
+                                         ((1, 8, 2, 3, 9001, False), True), ((1, 16, 2, 1, 9001, True), True)])
+def test_scratch_is_taken_only_where_the_plan_splits(b200, seed, case, splits):
+    # The split plan's scratch is some 38 MB; beside it a call allocates out and lse, each
+    # rounded up to a block of at most 2 MB more.
+    import torch
+
+    q, k, v, _ = make(case, seed=32)
+    seed.grouped_attention(q, k, v, case[5])
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out, lse = seed.grouped_attention(q, k, v, case[5])
+    taken = torch.cuda.max_memory_allocated() - before
+    results = out.numel() * 2 + lse.numel() * 4
+    scratch = b200.workspace(0).numel()
+    assert b200.grouped_plan(*case)[0] == (1 if splits else 0)
+    assert taken >= results + scratch if splits else taken <= results + (4 << 20)
