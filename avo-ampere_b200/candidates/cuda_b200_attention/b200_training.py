@@ -163,6 +163,22 @@ def _refuse_capture(what: str) -> None:
                            "capture the call under torch.no_grad() and its *_backward call")
 
 
+@functools.cache
+def _forward_ad():
+    import torch.autograd.forward_ad as forward_ad
+
+    return forward_ad
+
+
+def _refuse_tangents(what: str, *tensors) -> None:
+    """Raises if one of the tensors carries a tangent of forward-mode differentiation, which the
+    operators do not propagate (such a tensor need not require gradients)."""
+    forward_ad = _forward_ad()
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 _autograd_functions: dict[str, Any] = {}
 
 
@@ -206,10 +222,12 @@ def grouped_attention(q, k, v, causal: bool, *, softmax_scale: float | None = No
     keys j <= i + seq_kv - seq_q; a query that sees no key gets out 0 and lse -inf.
 
     With gradients enabled and an input that requires them, out is differentiable in q, k
-    and v (once; lse is not).  Such a call cannot be captured in a CUDA graph: capture the
+    and v (in reverse mode, once).  lse is not: what a loss computes from it adds nothing to
+    the gradients.  Such a call cannot be captured in a CUDA graph: capture the
     call under ``torch.no_grad()`` and ``attention_backward``."""
     torch = _torch()
     scale = _scale(softmax_scale)
+    _refuse_tangents("grouped_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         _attention_shape(q, k, v)
         with _on(q.get_device()):
@@ -236,9 +254,10 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool, *, softmax_scale: 
     ``attention_with_lse`` for equal shapes) returned for the same inputs and scale.  dk and
     dv sum over the query heads that share a key/value head.  All tensors are contiguous;
     the results go to ``dq``, ``dk``, ``dv`` where given (which overlap no other tensor of the
-    call).  The result does not depend on the
+    call) and carry no gradient themselves.  The result does not depend on the
     order in which the GPU runs the work: equal inputs give equal bits."""
     torch = _torch()
+    _refuse_tangents("attention_backward", dout, q, k, v, out, lse)
     batch, heads, kv_heads, seq_q, seq_kv = _attention_shape(q, k, v)
     scale = _scale(softmax_scale)
     index = q.get_device()
@@ -386,8 +405,10 @@ def qkv_norm_rope_backward(dq, dk, dv, qkv, cos, sin, *, q_weight=None, k_weight
 
     dq is bf16 [B, H, S, 128], dk and dv [B, Hkv, S, 128], contiguous; qkv and the other
     arguments are the forward's.  dqkv is a new contiguous tensor of qkv's shape, the weight
-    gradients are fp32 [128] (None without weights).  Equal inputs give equal bits."""
+    gradients are fp32 [128] (None without weights).  They carry no gradient themselves.
+    Equal inputs give equal bits."""
     torch = _torch()
+    _refuse_tangents("qkv_norm_rope_backward", dq, dk, dv, qkv, cos, sin, q_weight, k_weight)
     index = qkv.get_device()
     if not (_plain(dq, torch.bfloat16, index) and _plain(dk, torch.bfloat16, index)
             and _plain(dv, torch.bfloat16, index)):
@@ -479,12 +500,13 @@ def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=
     NaN and is reported by ``check_status()``.
 
     With gradients enabled and an input that requires them, the result is differentiable in
-    qkv and the weights (once), not in the tables, which must not require gradients then.
+    qkv and the weights (in reverse mode, once), not in the tables, which must not require gradients then.
     Such a call cannot be captured in a CUDA graph: capture the call under
     ``torch.no_grad()`` and ``qkv_norm_rope_backward``."""
     torch = _torch()
     sections = None if sections is None else tuple(map(int, sections))
     heads, kv_heads, interleaved = int(num_heads), int(num_kv_heads), bool(interleaved)
+    _refuse_tangents("qkv_norm_rope", qkv, cos, sin, q_weight, k_weight)
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise RuntimeError("qkv_norm_rope has no gradient for cos and sin: detach them")
     if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad)
