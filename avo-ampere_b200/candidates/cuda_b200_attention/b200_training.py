@@ -496,8 +496,9 @@ def qkv_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos, sin, *, q_weight=
 
     ``positions`` (int32 or int64) are the table rows: [S] or [B, S]; None is 0..S-1.  With
     ``sections`` (how many consecutive pairs each axis turns, up to 4 axes), positions are
-    [axes, S] or [axes, B, S].  A position outside the table makes the token's rotated values
-    NaN and is reported by ``check_status()``.
+    [axes, S] or [axes, B, S]; those of an axis that turns no pairs are not looked at.  A
+    position outside the table makes the token's rotated values NaN and is reported by
+    ``check_status()``.
 
     With gradients enabled and an input that requires them, the result is differentiable in
     qkv and the weights (in reverse mode, once), not in the tables, which must not require gradients then.

@@ -180,7 +180,8 @@ __device__ __forceinline__ long long row_at(const RopeParams& p, const Task& t, 
   return ((static_cast<long long>(t.batch) * (t.kind == 0 ? p.heads : p.kv_heads) + h) * p.seq + t.s) * kRow;
 }
 
-// The table rows of a token, one per axis; whether one of them lies outside (then row 0).
+// The table rows of a token, one per axis; whether one of them lies outside (then row 0).  The
+// position of an axis that owns no columns is not looked at: nothing is read for it.
 struct TableRows {
   long long row[kMaxAxes];
   bool bad;
@@ -191,7 +192,7 @@ __device__ __forceinline__ TableRows table_rows(const RopeParams& p, const Task&
 #pragma unroll
   for (int a = 0; a < kMaxAxes; ++a) {
     rows.row[a] = 0;
-    if (a < p.axes) {
+    if (a < p.axes && p.end[a] > (a > 0 ? p.end[a - 1] : 0)) {
       long long r = t.s;
       if (p.pos != nullptr) {
         const long long at = a * p.pos_sa + t.batch * p.pos_sb + t.s * p.pos_ss;

@@ -234,9 +234,10 @@ int avo_b200_attn_bwd(const void* dout, const void* q, const void* k, const void
  * values at axis * pos_axis_stride + batch * pos_batch_stride + token * pos_token_stride
  * elements.  axes = 1: one position per token.  axes = 2..4: one per axis (time, height,
  * width, ...); axis a turns sections[a] consecutive pairs (host array; the sections sum to
- * rotary_dim / 2).  A position outside the table sets AVO_B200_STATUS_POSITION and gives
- * NaN in the token's rotated values.  batch * seq is limited to 2^31 - 1 tokens, and
- * pairs of tokens times their runs of up to 16 heads of a kind to 2^31 - 1 as well.
+ * rotary_dim / 2; the positions of an axis of no pairs are not looked at).  A position outside
+ * the table sets AVO_B200_STATUS_POSITION and gives NaN in the token's rotated values.
+ * batch * seq is limited to 2^31 - 1 tokens, and pairs of tokens times their runs of up to 16
+ * heads of a kind to 2^31 - 1 as well.
  * No reference counterpart (the reference starts at q, k, v).
  */
 int avo_b200_qkv_norm_rope(const void* qkv, long long batch_stride, long long token_stride, void* q, void* k,
