@@ -219,7 +219,8 @@ def grouped_attention(q, k, v, causal: bool, *, softmax_scale: float | None = No
     q is bf16 [B, H, seq_q, 128], k and v [B, Hkv, seq_kv, 128] with H a multiple of Hkv
     (query head h reads head h // (H // Hkv)), all contiguous; out is like q, lse fp32
     [B, H, seq_q] (natural log).  ``causal`` aligns the sequences at their ends: query i sees
-    keys j <= i + seq_kv - seq_q; a query that sees no key gets out 0 and lse -inf.
+    keys j <= i + seq_kv - seq_q; a query that sees no key gets out 0 and lse -inf, one that
+    sees a NaN score or a score of +infinity gets NaN in both.
 
     With gradients enabled and an input that requires them, out is differentiable in q, k
     and v (in reverse mode, once).  lse is not: what a loss computes from it adds nothing to

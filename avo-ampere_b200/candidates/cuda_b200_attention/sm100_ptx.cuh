@@ -371,11 +371,29 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-// Three-input maximum (sm_100).
+// Maximum of three (sm_100) and of two; with kNan a NaN among them gives NaN, without it is
+// passed over.
+template <bool kNan>
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  if constexpr (kNan)
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  else
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+template <bool kNan>
+__device__ __forceinline__ float fmax2(float a, float b) {
+  if constexpr (!kNan) return fmaxf(a, b);
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// a > 0; with kNan also true for NaN.
+template <bool kNan>
+__device__ __forceinline__ bool above_zero(float a) {
+  return kNan ? !(a <= 0.f) : a > 0.f;
 }
 
 // Packed pairs of fp32 in one 64-bit register (sm_100 f32x2 arithmetic).

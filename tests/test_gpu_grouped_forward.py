@@ -122,3 +122,72 @@ def test_scratch_is_taken_only_where_the_plan_splits(b200, seed, case, splits):
     scratch = b200.workspace(0).numel()
     assert b200.grouped_plan(*case)[0] == (1 if splits else 0)
     assert taken >= results + scratch if splits else taken <= results + (4 << 20)
+
+
+# NaN: in whole items, in lists, and in the first and in a later piece of split work.
+NAN_CASES = [((1, 2, 1, 40, 40, True), (0, 1, 2, 17, 39)), ((1, 2, 2, 300, 300, True), (0, 1, 129, 288)),
+             ((2, 74, 37, 300, 300, True), (16, 130)), ((1, 2, 1, 1, 1, False), (0,)),
+             ((1, 8, 2, 3, 9001, False), (0, 1, 4800, 9000))]
+
+
+@pytest.mark.parametrize("case,places", NAN_CASES)
+def test_nan_reaches_exactly_the_rows_that_see_it(b200, seed, case, places):
+    # A score that is NaN makes its row NaN, LSE included, wherever its key lies in a tile; rows
+    # that do not see the key, or belong to another query, keep their bits.
+    import torch
+
+    q, k, v, _ = make(case, seed=33)
+    seq_q, seq_kv, causal = case[3:]
+    clean, clean_lse = seed.grouped_attention(q, k, v, causal)
+    row = torch.arange(seq_q, device="cuda")
+    for at in places:
+        for what in ("key", "query"):
+            x = (k if what == "key" else q).clone()
+            if what == "query" and at >= seq_q:
+                continue
+            x[-1, -1, at, 5] = float("nan")
+            out, lse = seed.grouped_attention(*((q, x) if what == "key" else (x, k)), v, causal)
+            bad = torch.zeros(case[0], case[1], seq_q, dtype=torch.bool, device="cuda")
+            if what == "query":
+                bad[-1, -1, at] = True
+            else:
+                bad[-1, -(case[1] // case[2]):] = row + seq_kv - seq_q >= at if causal else True
+            torch.cuda.synchronize()
+            assert torch.equal(torch.isnan(out).all(-1), bad) and torch.equal(torch.isnan(lse), bad), (what, at)
+            assert torch.equal(out[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad]), (what, at)
+    b200.check_status(q.device)
+
+
+@pytest.mark.parametrize("case", [(1, 2, 1, 40, 40, True), (1, 8, 2, 3, 9001, False)])
+def test_infinite_scores_make_a_row_nan(b200, seed, case):
+    # Scores of +infinity, as the softmax of the definition: infinity - infinity is NaN.
+    import torch
+
+    q, k, v, _ = make(case, seed=34)
+    q[0, 0, 2, 7] = float("inf")
+    out, lse = seed.grouped_attention(q, k.abs(), v, case[5])
+    torch.cuda.synchronize()
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    bad[0, 0, 2] = True
+    assert torch.equal(torch.isnan(out).all(-1), bad) and torch.equal(torch.isnan(lse), bad)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 150])
+def test_gradients_of_a_nan_query(b200, seed, at):
+    # Its own gradient is NaN, no gradient of a key that it sees is finite; the other queries'
+    # gradients and the other key/value heads keep their bits.
+    import torch
+
+    q, k, v, do = make((1, 4, 2, 300, 300, True), seed=35)
+    out, lse = seed.grouped_attention(q, k, v, True)
+    clean = seed.attention_backward(do, q, k, v, out, lse, True)
+    q[0, 3, at, 5] = float("nan")
+    out, lse = seed.grouped_attention(q, k, v, True)
+    dq, dk, dv = seed.attention_backward(do, q, k, v, out, lse, True)
+    torch.cuda.synchronize()
+    b200.check_status(q.device)
+    assert bool(torch.isnan(dq[0, 3, at]).all())
+    dq[0, 3, at] = clean[0][0, 3, at]
+    assert torch.equal(dq, clean[0])
+    for got, want in ((dk, clean[1]), (dv, clean[2])):
+        assert torch.equal(got[0, 0], want[0, 0]) and not bool(torch.isfinite(got[0, 1, :at + 1]).any())
