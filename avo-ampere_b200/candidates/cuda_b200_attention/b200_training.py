@@ -179,6 +179,13 @@ def _refuse_tangents(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
+def _incoming(grad):
+    """A gradient as autograd hands it over, contiguous and on the kernels' 16-byte grid: a slice of
+    a larger gradient (torch.cat's) can be contiguous and off it."""
+    grad = grad.contiguous()
+    return grad if grad.data_ptr() % 16 == 0 else grad.clone()
+
+
 _autograd_functions: dict[str, Any] = {}
 
 
@@ -206,7 +213,7 @@ def _attention_function():
             q, k, v, out, lse = ctx.saved_tensors
             with _on(q.get_device()):
                 _refuse_capture("the backward of grouped_attention")
-            grads = attention_backward(dout.contiguous(), q, k, v, out, lse, ctx.causal, softmax_scale=ctx.scale)
+            grads = attention_backward(_incoming(dout), q, k, v, out, lse, ctx.causal, softmax_scale=ctx.scale)
             return (*grads, None, None)
 
     _autograd_functions["attention"] = GroupedAttention
@@ -474,7 +481,7 @@ def _norm_rope_function():
             with _on(qkv.get_device()):
                 _refuse_capture("the backward of qkv_norm_rope")
             dqkv, dqw, dkw = qkv_norm_rope_backward(
-                dq.contiguous(), dk.contiguous(), dv.contiguous(), qkv, cos, sin, q_weight=q_weight,
+                _incoming(dq), _incoming(dk), _incoming(dv), qkv, cos, sin, q_weight=q_weight,
                 k_weight=k_weight, positions=positions, sections=sections, eps=eps, interleaved=interleaved)
             if dqw is not None:
                 dqw, dkw = dqw.to(q_weight.dtype), dkw.to(k_weight.dtype)
