@@ -1,5 +1,5 @@
 // C-ABI entry points of the attention gradient (declared in include/avo_b200_attn.h): argument checks, tensor maps
-// and the three launches of attn_bwd.cuh.
+// and the launches of attn_bwd.cuh.
 #include <algorithm>
 #include <atomic>
 #include <climits>

@@ -6,9 +6,10 @@
 // dK and dV summed over the query heads that share a key/value head.  The probabilities are
 // recomputed from Q, K and the LSE the forward saved.
 //
-// Three launches.  stats_kernel writes -LSE*log2(e) and -delta per query row.  Then one
-// kernel template runs twice over 128 x 128 tiles, each time with one side of the tile
-// stationary and the other streamed through shared memory:
+// Three launches, and a fourth (join_kernel) where work is split.  stats_kernel writes
+// -LSE*log2(e) and -delta per query row.  Then one kernel template runs twice over 128 x 128
+// tiles, each time with one side of the tile stationary and the other streamed through shared
+// memory:
 //
 //             rows (M)   stationary X1, X2   streamed Y1, Y2   accumulators in TMEM
 //   dK/dV     keys       K, V                Q, dO             dK += dS^T Q, dV += P^T dO
@@ -182,7 +183,7 @@ struct BwdParams {
   int causal;
   int offset;              // causal: key j is visible to query i iff j <= i + offset
   float scale, scale_log2;
-  uint32_t* claims;        // null (one item per CTA at most), or gridDim.x zeros: places taken
+  uint32_t* claims;        // null (place = CTA number), or gridDim.x zeros: places taken
   int test_skip_load;
   // An item is a stationary tile; with split > 1 it is cut into that many pieces along the
   // streamed tiles, each a unit of its own whose sums go to part1 / part2 in fp32
@@ -285,7 +286,11 @@ struct Items {
           n = min(p.nkv, (max(end, 0) + kTile - 1) >> 7);
         }
       } else {
-        // The first query that sees the tile's first key; past the last query: no tiles.
+        // The tile of the first query that sees the tile's first key.  The bounds by nq never
+        // bind: offset is seq_kv - seq_q, so the last query sees every key.  They stay for what
+        // the compiler makes of them, which without them keeps more of this instance's
+        // registers in memory (measured on B200, with / without: B1 H16 Hkv2 Q777 KV5003 104.4 /
+        // 106.3 us, B1 H4 Hkv2 Q300 KV900 20.1 / 20.7, B1 H8 Hkv2 S2048 39.6 / 39.9, causal).
         if (p.causal) t0 = min(max(0, tile * kTile - p.offset) >> 7, p.nq);
         if (p.causal && tile * kTile - p.offset >= p.seq_q) t0 = p.nq;
         n = (p.nq - t0) * p.group;
@@ -447,9 +452,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     grid_dependency_wait();
     grid_launch_dependents();
   }
-  // CTAs with several items take their place in the order of items by multiprocessor (the next
-  // free one, should two CTAs ask for the same), and dQ counts from the other end.  Then a
-  // multiprocessor that has one item more of dK/dV has the fewest of dQ, and the two of a pair
+  // With a unit for every multiprocessor, CTAs take their place in the order of items by
+  // multiprocessor (the next free one, should two CTAs ask for the same), and dQ counts from
+  // the other end.  Then a multiprocessor that has one item more of dK/dV has the fewest of dQ, and the two of a pair
   // (a TPC) change from one pass to the other at the same time: while they run different
   // kernels, both take up to twice as long (the pair seems to share its instruction cache).
   // Measured on B200, B1 H16 S4096: both passes one after the other 391 to 413 us, at once
@@ -884,10 +889,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   } else if (warp == kIssuerWarp) {
     regs_decrease<kBwdRegsOther>();
     // ------------------------------------------------------------ MMA issuer
-    // The issuing lane is chosen by elect.sync: with `lane == 0` the compiler moves every
-    // operand of every MMA to uniform registers one lane at a time, and issuing became the
-    // limit (measured on B200, B1 H16 S4096: 3324 and 2731 cycles per tile pair of the two
-    // passes, 2814 and 2104 with elect.sync).
+    // The issuing lane is chosen by elect.sync: with `lane == 0` issuing was the limit
+    // (measured on B200, B1 H16 S4096: 3324 and 2731 cycles per tile pair of the two passes,
+    // 2814 and 2104 with elect.sync).
     const bool leader = elect_one();
     const uint32_t tT1 = tmem + kColT1, tT2 = tmem + kColT2, tA1 = tmem + kColAcc1, tA2 = tmem + kColAcc2;
     const uint32_t tDs = tmem + kColDs, tX1 = tmem + kColX1;

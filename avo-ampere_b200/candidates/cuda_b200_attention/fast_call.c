@@ -1,9 +1,10 @@
 /* CPython binding of the C-ABI entries that are called once per operator call: first
- * avo_b200_attn_fwd_ws, for attention(); the entries of the training side follow below.  Small problems are bound by host time per call (the B1 H4 S512 case of the
- * scorer runs ~15 us of GPU work per launch); a ctypes call with fifteen arguments costs
- * ~2 us of argument conversion, a METH_FASTCALL function a fraction of that.  The function
- * address comes from the library ctypes already loaded (bind), so this module links to
- * nothing but Python and calls exactly the same native entry.
+ * avo_b200_attn_fwd_ws, for attention(); the entries of the training side follow below.
+ * Small problems are bound by host time per call (the B1 H4 S512 case of the scorer runs
+ * ~15 us of GPU work per launch); a ctypes call with fifteen arguments costs ~2 us of argument
+ * conversion, a METH_FASTCALL function a fraction of that.  The function address comes from
+ * the library ctypes already loaded (bind), so this module links to nothing but Python and
+ * calls exactly the same native entry.
  *
  * fwd_ws(q, k, v, o, lse_or_None, batch, heads, seq, head_dim, causal, scale,
  *        workspace, workspace_bytes, status, stream) -> int status code

@@ -106,7 +106,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// Two packed fp32 pairs from shared memory (16-byte aligned).
 // Per-thread asynchronous copies to shared memory, both addresses aligned to their size; a
 // commit closes a group, wait<n> leaves at most the last n groups in flight.
 template <int kBytes>
@@ -126,6 +125,7 @@ __device__ __forceinline__ uint32_t sm_id() {
   return id;
 }
 
+// Two packed fp32 pairs from shared memory (16-byte aligned).
 __device__ __forceinline__ void lds_f2x2(uint32_t addr, uint64_t& a, uint64_t& b) {
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
 }

@@ -207,9 +207,9 @@ int avo_b200_attn_fwd_grouped_plan(int batch, int heads, int kv_heads, int seq_q
  * bits in every call: nothing is accumulated in an order that can change.
  * dq, dk, dv must be 32-byte aligned, the inputs 16-byte aligned.
  * workspace: device memory of avo_b200_attn_bwd_workspace_size() bytes (a function of the
- * sizes alone, needs no device), 256-byte aligned, uninitialised; used from the launch until the call's work on the stream is done.  Calls
- * that may overlap in time need a workspace each.  No reference counterpart (the reference
- * scores the forward only).
+ * sizes alone, needs no device), 256-byte aligned, uninitialised; used from the launch until
+ * the call's work on the stream is done.  Calls that may overlap in time need a workspace
+ * each.  No reference counterpart (the reference scores the forward only).
  */
 int avo_b200_attn_bwd_workspace_size(int batch, int heads, int kv_heads, int seq_q, int seq_kv, int causal,
                                      size_t* bytes);
