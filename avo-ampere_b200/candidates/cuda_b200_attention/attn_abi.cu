@@ -485,8 +485,8 @@ extern "C" const char* avo_b200_strerror(int code) {
     case AVO_B200_ETENSORMAP: return "tensor map encoding failed";
     case AVO_B200_EDRIVER: return "driver entry point cuTensorMapEncodeTiled unavailable";
     case AVO_B200_EREGS:
-      return "attention kernel built with an unexpected register count (the setmaxnreg split needs 168 per "
-             "thread at launch); rebuild the library";
+      return "attention kernel built with an unexpected register count (the setmaxnreg splits need 168 per "
+             "thread at launch in the forward, 80 in the gradient); rebuild the library";
     case AVO_B200_ETOOBIG:
       return "problem too large for the no-allocation entry point (batch*heads*seq > 16384 rows)";
     default: return "unknown error";
