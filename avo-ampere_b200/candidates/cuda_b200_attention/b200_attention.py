@@ -228,9 +228,13 @@ _status_addresses: dict[int, int] = {}
 
 
 def status_address(index: int) -> int:
-    """Address of device ``index``'s status word (it lives as long as the process)."""
+    """Address of device ``index``'s status word (it lives as long as the process).  Raises where the word would
+    be created inside a CUDA-graph capture: it would hold anything until the first replay, and be cleared by
+    every replay."""
     address = _status_addresses.get(index)
     if address is None:
+        if index not in _status_words and _torch().cuda.is_current_stream_capturing():
+            raise RuntimeError(f"the first call on device {index} cannot be captured in a CUDA graph")
         address = _status_addresses[index] = status_word(index).data_ptr()
     return address
 

@@ -191,3 +191,18 @@ def test_gradients_of_a_nan_query(b200, seed, at):
     assert torch.equal(dq, clean[0])
     for got, want in ((dk, clean[1]), (dv, clean[2])):
         assert torch.equal(got[0, 0], want[0, 0]) and not bool(torch.isfinite(got[0, 1, :at + 1]).any())
+
+
+def test_offsets_past_32_bits_within_the_derived_bounds(b200, seed):
+    # q and out have more than 2^31 elements; the last heads of the last batch entry.
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of device memory")
+    q, k, v, _ = make((16, 1024, 256, 1100, 1100, True), seed=36)
+    assert q.numel() > 2**31
+    out, lse = seed.grouped_attention(q, k, v, True)
+    torch.cuda.synchronize()
+    b200.check_status(q.device)
+    few = (t[-1:, h] for t, h in ((q, slice(-8, None)), (k, slice(-2, None)), (v, slice(-2, None))))
+    check(b200, *few, True, out[-1:, -8:], lse[-1:, -8:])
