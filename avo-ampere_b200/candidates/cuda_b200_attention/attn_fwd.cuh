@@ -226,13 +226,16 @@ __device__ __forceinline__ void issue_pv_half(uint32_t d_tmem, uint32_t p_tmem, 
 __device__ __forceinline__ float u2f(uint32_t x) { return __uint_as_float(x); }
 __device__ __forceinline__ uint32_t f2u(float x) { return __float_as_uint(x); }
 
+// 2^x on the FMA pipe.  Its floor is 2^-125 with degree 3; with degree 5 it is 2^-149, which is 0
+// as bf16: a hidden key adds nothing to the output then, however large its value.  (A test and a
+// select in place of the lower clamp: 1.3 to 3.4 % more time on B200.)
 template <int kDegree>
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& r0, float& r1) {
+__device__ __forceinline__ void exp2_poly(float x0, float x1, float& r0, float& r1) {
   static_assert(kDegree == 3 || kDegree == 5, "polynomials of degree 3 and 5");
   if constexpr (kDegree == 3)
-    exp2_poly_x2(x2, r0, r1);
+    exp2_poly_x2(f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f)), r0, r1);
   else
-    exp2_poly5_x2(x2, r0, r1);
+    exp2_poly5_x2(f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f)), r0, r1);
 }
 
 // Whether a kernel carries a NaN score to its row: through the row's maximum, which then is NaN
@@ -249,8 +252,8 @@ constexpr bool kCarriesNan = kDegree == 5;
 // kEmuPairsPer8 of every 8 pairs go through the FMA-pipe exp2 (exp2_poly_x2) to
 // offload the MUFU unit; the split is fixed at compile time, so the whole half is one
 // straight-line block in which MUFU and FMA chains interleave.  A masked (-inf) score
-// gives exactly 0 on the MUFU path and 2^-125 on the FMA path: negligible against any
-// row that sees a key (the row sum is >= 1), and a row that sees none is zeroed in
+// gives exactly 0 on the MUFU path and the floor of exp2_poly on the FMA path: negligible
+// against any row that sees a key (the row sum is >= 1), and a row that sees none is zeroed in
 // the epilogue.
 template <int kDegree>
 __device__ __forceinline__ void exp_half(const uint32_t (&sa)[32], const uint32_t (&sb)[32],
@@ -266,7 +269,7 @@ __device__ __forceinline__ void exp_half(const uint32_t (&sa)[32], const uint32_
       float x0, x1, p0, p1;
       f2_unpack(x2, x0, x1);
       if (((e >> 1) & 7) < kEmuPairsPer8) {
-        exp2_poly<kDegree>(f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f)), p0, p1);
+        exp2_poly<kDegree>(x0, x1, p0, p1);
       } else {
         p0 = ex2_approx(x0);
         p1 = ex2_approx(x1);
@@ -301,7 +304,7 @@ __device__ __forceinline__ float exp_half_max(const uint32_t (&s)[4][32], uint64
     float x0, x1, p0, p1;
     f2_unpack(x2, x0, x1);
     if ((q & 7) < kEmuPairsPer8) {
-      exp2_poly<kDegree>(f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f)), p0, p1);
+      exp2_poly<kDegree>(x0, x1, p0, p1);
     } else {
       p0 = ex2_approx(x0);
       p1 = ex2_approx(x1);

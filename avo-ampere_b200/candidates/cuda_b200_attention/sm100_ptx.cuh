@@ -451,7 +451,9 @@ __device__ __forceinline__ void exp2_poly_x2(uint64_t x2, float& r0, float& r1) 
   r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
-// The same with the polynomial of degree 5 (relative error < 2.2e-7, evaluated in fp32).
+// The same with the polynomial of degree 5 (relative error < 2.2e-7, evaluated in fp32).  Its
+// inputs start at -127: the polynomial is above 1 there, so the exponent does not wrap, and
+// -127 gives its last bits as a subnormal, 2^-149 (below 2^-126 the result is off by up to 2^-127).
 __device__ __forceinline__ void exp2_poly5_x2(uint64_t x2, float& r0, float& r1) {
   const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
   const uint64_t neg_magic = f2_pack(-12582912.0f, -12582912.0f);

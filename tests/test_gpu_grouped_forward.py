@@ -206,3 +206,19 @@ def test_offsets_past_32_bits_within_the_derived_bounds(b200, seed):
     b200.check_status(q.device)
     few = (t[-1:, h] for t, h in ((q, slice(-8, None)), (k, slice(-2, None)), (v, slice(-2, None))))
     check(b200, *few, True, out[-1:, -8:], lse[-1:, -8:])
+
+
+@pytest.mark.parametrize("case", [(1, 2, 1, 130, 130, True), (1, 4, 2, 90, 300, True), (2, 74, 37, 300, 300, True)])
+def test_hidden_values_add_nothing_however_large(b200, seed, case):
+    # Rows that do not see the last keys keep their bits when those hold the type's largest and
+    # lowest values; 2^-125 of them would be 8.
+    import torch
+
+    q, k, v, _ = make(case, seed=37)
+    out, lse = seed.grouped_attention(q, k, v, True)
+    few = 40
+    v[:, :, -few:, ::2] = torch.finfo(torch.bfloat16).max
+    v[:, :, -few:, 1::2] = torch.finfo(torch.bfloat16).min
+    got, got_lse = seed.grouped_attention(q, k, v, True)
+    torch.cuda.synchronize()
+    assert torch.equal(got[:, :, :-few], out[:, :, :-few]) and torch.equal(got_lse, lse)
