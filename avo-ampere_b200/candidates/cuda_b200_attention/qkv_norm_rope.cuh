@@ -20,9 +20,9 @@
 // the load and one rounding to bf16.  The weights' gradients are summed per thread, then per
 // CTA, then over CTAs by a second kernel, each in a fixed order: equal inputs give equal bits.
 //
-// Memory bandwidth bounds both.  Measured on B200, B4 S4096 H16 Hkv4 (inputs not in L2): the
-// forward 34.8 us, 5.85 TB/s, against 31 at the rate of a plain copy; the gradient 56.7 us,
-// 5.07 TB/s, against 44.  The gradient's issue slots are 60 % busy with a quarter of the warps
+// Memory bandwidth bounds both.  Measured on B200, B4 S4096 H16 Hkv4 (inputs not in L2), calls
+// back to back / among other work: the forward 33.8 / 35.1 us (5.8 TB/s) against 31 at the rate
+// of a plain copy; the gradient 56.5 / 59.2 us (4.9 TB/s) against 44.  The gradient's issue slots are 60 % busy with a quarter of the warps
 // resident (its registers), so computing and fetching do not overlap fully.
 #pragma once
 
